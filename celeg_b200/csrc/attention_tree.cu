@@ -1,0 +1,389 @@
+// Attention of a tree of drafted tokens over the paged cache (see attention_tree.cuh): the general kernel, the join of split
+// keys, and the entry point that chooses.
+//
+// The general kernel takes float32 and bfloat16, any head size up to 256 and any page size. Everything is float32: a block has
+// 32 rows (node, query head of a group) of one kv head and walks its keys 64 at a time. 128 threads: for the scores a thread
+// has 4 rows x 4 keys, for the weighted sum 4 rows x 4 columns of every 64, operands from shared memory four numbers at a time.
+#include "attention_tree.cuh"
+
+namespace celeg_b200 {
+
+constexpr int kSimtThreads = 128;
+constexpr int kSimtRows = 32;
+constexpr int kSimtKeys = 64;
+
+__host__ __device__ inline int simt_pitch(int head_dim) {
+    // rows of 16-byte pieces, eight consecutive rows in different banks
+    const int four = (head_dim + 3) / 4 * 4;
+    return four % 32 == 0 ? four + 4 : four;
+}
+
+inline size_t simt_smem(int head_dim, int columns) {
+    const size_t q_k = (size_t)(kSimtRows + kSimtKeys) * simt_pitch(head_dim);
+    return (q_k + (size_t)kSimtKeys * columns + kSimtRows * (kSimtKeys + 4)) * sizeof(float) + kSimtKeys * (sizeof(int) + sizeof(long long));
+}
+
+template <typename A>
+__device__ __forceinline__ float4 load_four(const A* p);
+template <>
+__device__ __forceinline__ float4 load_four<float>(const float* p) { return *reinterpret_cast<const float4*>(p); }
+template <>
+__device__ __forceinline__ float4 load_four<__nv_bfloat16>(const __nv_bfloat16* p) {
+    const uint2 raw = *reinterpret_cast<const uint2*>(p);
+    const float2 lo = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.x));
+    const float2 hi = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.y));
+    return make_float4(lo.x, lo.y, hi.x, hi.y);
+}
+
+// A row of `head_dim` numbers in global memory, four of them from column c on (zeros past the end).
+template <typename A, bool FOUR>
+__device__ __forceinline__ float4 row_four(const A* row, int c, int head_dim) {
+    if (FOUR) return load_four<A>(row + c);
+    float4 v;
+    v.x = c < head_dim ? to_float(row[c]) : 0.0f;
+    v.y = c + 1 < head_dim ? to_float(row[c + 1]) : 0.0f;
+    v.z = c + 2 < head_dim ? to_float(row[c + 2]) : 0.0f;
+    v.w = c + 3 < head_dim ? to_float(row[c + 3]) : 0.0f;
+    return v;
+}
+
+// COLUMNS: columns of the output in units of 64 (head_dim <= 64 * COLUMNS). FOUR: rows are read four numbers at a time.
+template <typename A, int COLUMNS, bool FOUR>
+__global__ void __launch_bounds__(kSimtThreads) attention_tree_simt_kernel(const TreeParams p) {
+    extern __shared__ __align__(16) float smem[];
+    const int d = p.head_dim, pitch = simt_pitch(d);
+    float* q_s = smem;                                      // [rows][pitch]
+    float* k_s = q_s + kSimtRows * pitch;                   // [keys][pitch]
+    float* v_s = k_s + kSimtKeys * pitch;                   // [keys][64 * COLUMNS]
+    float* w_s = v_s + kSimtKeys * 64 * COLUMNS;            // [rows][keys + 4]
+    long long* offset_s = reinterpret_cast<long long*>(w_s + kSimtRows * (kSimtKeys + 4));      // [keys], -1: no such key
+    int* position_s = reinterpret_cast<int*>(offset_s + kSimtKeys);                             // [keys]
+    __shared__ int lowest_s;
+
+    const int tid = threadIdx.x, kx = tid & 15, ry = tid >> 4;
+    const int span = blockIdx.z, split = blockIdx.x;
+    const int tiles = (p.max_nodes * p.group + kSimtRows - 1) / kSimtRows;
+    const int kvh = blockIdx.y / tiles, row0 = (blockIdx.y % tiles) * kSimtRows;
+    const TreeSpan s = tree_span(p, span);
+    const int rows = s.nodes * p.group;
+    if (row0 >= rows) return;
+    const int* table = p.block_table + (size_t)span * p.table_stride;
+    const A* q = static_cast<const A*>(p.q);
+
+    // the keys of this block: from the first that any of its rows sees, in `splits` pieces of whole tiles
+    if (tid == 0) lowest_s = 0x7fffffff;
+    __syncthreads();
+    if (p.window && tid < kSimtRows && row0 + tid < rows) atomicMin(&lowest_s, p.positions[s.begin + (row0 + tid) / p.group]);
+    for (int i = tid; i < kSimtRows * (pitch / 4); i += kSimtThreads) {
+        const int r = i / (pitch / 4), c = (i % (pitch / 4)) * 4, row = row0 + r;
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (row < rows && c < d)
+            v = row_four<A, FOUR>(q + (size_t)(s.begin + row / p.group) * p.q_row_stride + (size_t)(kvh * p.group + row % p.group) * d, c, d);
+        *reinterpret_cast<float4*>(q_s + r * pitch + c) = v;
+    }
+    __syncthreads();
+    const int first = p.window ? tree_first_place(p, s, lowest_s) : 0, last = s.context + s.nodes;
+    const int per_split = ((last - first + p.splits - 1) / p.splits + kSimtKeys - 1) / kSimtKeys * kSimtKeys;
+    const long long from = (long long)first + (long long)split * per_split;
+    const int end = (int)min((long long)last, from + per_split);
+
+    int node_position[4];
+    const unsigned* mask[4];
+    float run_max[4], run_sum[4], acc[4][COLUMNS][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int node = s.begin + min(row0 + ry * 4 + i, rows - 1) / p.group;
+        node_position[i] = p.window ? p.positions[node] : 0;
+        mask[i] = p.ancestors + (size_t)node * p.words;
+        run_max[i] = -INFINITY;
+        run_sum[i] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < COLUMNS; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][j][e] = 0.0f;
+    }
+
+    for (long long base = from; base < end; base += kSimtKeys) {
+        const int key0 = (int)base, count = min(kSimtKeys, end - key0);
+        if (tid < kSimtKeys) {
+            const int place = key0 + tid;
+            long long offset = -1;
+            int position = place;
+            if (tid < count) {
+                const int page = tree_page(p, table, place);
+                if (page >= 0) offset = (long long)page * p.page_stride + ((long long)kvh * p.page_tokens + place % p.page_tokens) * d;
+                if (p.window && place >= s.context) position = p.positions[s.begin + place - s.context];
+            }
+            offset_s[tid] = offset;
+            position_s[tid] = position;
+        }
+        __syncthreads();
+        const A* k = static_cast<const A*>(p.k_cache);
+        const A* v = static_cast<const A*>(p.v_cache);
+        for (int i = tid; i < kSimtKeys * (pitch / 4); i += kSimtThreads) {
+            const int r = i / (pitch / 4), c = (i % (pitch / 4)) * 4;
+            const long long offset = offset_s[r];
+            *reinterpret_cast<float4*>(k_s + r * pitch + c) =
+                offset >= 0 && c < d ? row_four<A, FOUR>(k + offset, c, d) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+        for (int i = tid; i < kSimtKeys * 16 * COLUMNS; i += kSimtThreads) {
+            const int r = i / (16 * COLUMNS), c = (i % (16 * COLUMNS)) * 4;
+            const long long offset = offset_s[r];
+            *reinterpret_cast<float4*>(v_s + r * 64 * COLUMNS + c) =
+                offset >= 0 && c < d ? row_four<A, FOUR>(v + offset, c, d) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+        __syncthreads();
+
+        float score[4][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) score[i][j] = 0.0f;
+        for (int c = 0; c < d; c += 4) {
+            float4 a[4], b[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const float4*>(q_s + (ry * 4 + i) * pitch + c);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const float4*>(k_s + (kx + 16 * j) * pitch + c);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    score[i][j] = fmaf(a[i].x, b[j].x, score[i][j]);
+                    score[i][j] = fmaf(a[i].y, b[j].y, score[i][j]);
+                    score[i][j] = fmaf(a[i].z, b[j].z, score[i][j]);
+                    score[i][j] = fmaf(a[i].w, b[j].w, score[i][j]);
+                }
+        }
+        // every row sees every key of the tile, unless the tile reaches into the tree, the window's edge or a missing page
+        const bool whole = __syncthreads_and(p.window == 0 && key0 + kSimtKeys <= s.context && (tid >= kSimtKeys || offset_s[tid] >= 0));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float x = score[i][j];
+                x = p.cap_out > 0.0f ? p.cap_out * tanhf(x * p.cap_in) : x * p.scale;
+                const int at = kx + 16 * j;
+                if (!whole && (offset_s[at] < 0 || !tree_sees(p, s, mask[i], node_position[i], key0 + at, position_s[at]))) x = -INFINITY;
+                score[i][j] = x;
+                top = fmaxf(top, x);
+            }
+#pragma unroll
+            for (int lanes = 8; lanes > 0; lanes >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, lanes));
+            const float new_max = fmaxf(run_max[i], top);
+            const float base_max = new_max == -INFINITY ? 0.0f : new_max;
+            const float factor = expf(run_max[i] - base_max);            // (-inf - 0: 0, of sums that are 0)
+            run_max[i] = new_max;
+            float sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float w = expf(score[i][j] - base_max);
+                w_s[(ry * 4 + i) * (kSimtKeys + 4) + kx + 16 * j] = w;
+                sum += w;
+            }
+            run_sum[i] = run_sum[i] * factor + sum;                      // (this lane's share of the row)
+#pragma unroll
+            for (int j = 0; j < COLUMNS; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i][j][e] *= factor;
+        }
+        __syncwarp();                        // (a warp's 8 rows of weights are read by this warp alone)
+        for (int n = 0; n < count; n += 4) {
+            float w[4][4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float4 four = *reinterpret_cast<const float4*>(w_s + (ry * 4 + i) * (kSimtKeys + 4) + n);
+                w[i][0] = four.x, w[i][1] = four.y, w[i][2] = four.z, w[i][3] = four.w;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+#pragma unroll
+                for (int j = 0; j < COLUMNS; ++j) {
+                    const float4 x = *reinterpret_cast<const float4*>(v_s + (n + e) * 64 * COLUMNS + j * 64 + kx * 4);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        // (a masked key's weight is 0: its value, whatever it is, must not reach the row)
+                        if (!whole && w[i][e] == 0.0f) continue;
+                        acc[i][j][0] = fmaf(w[i][e], x.x, acc[i][j][0]);
+                        acc[i][j][1] = fmaf(w[i][e], x.y, acc[i][j][1]);
+                        acc[i][j][2] = fmaf(w[i][e], x.z, acc[i][j][2]);
+                        acc[i][j][3] = fmaf(w[i][e], x.w, acc[i][j][3]);
+                    }
+                }
+            }
+        }
+        __syncthreads();
+    }
+
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float sum = run_sum[i];
+#pragma unroll
+        for (int lanes = 8; lanes > 0; lanes >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, lanes);
+        const int row = row0 + ry * 4 + i;
+        if (row >= rows) continue;
+        const int head = kvh * p.group + row % p.group;
+        const size_t unit = (size_t)(s.begin + row / p.group) * p.q_heads + head;
+        if (p.splits > 1) {
+            if (kx == 0) {
+                p.part_ml[(unit * p.splits + split) * 2] = run_max[i] * 1.4426950408889634f;
+                p.part_ml[(unit * p.splits + split) * 2 + 1] = sum;
+            }
+            if (run_max[i] == -INFINITY) continue;
+        }
+        float inv = 1.0f;
+        if (p.splits == 1) {
+            if (p.sinks && sum > 0.0f) sum += expf(p.sinks[head] - run_max[i]);
+            inv = run_max[i] == -INFINITY ? 0.0f : 1.0f / sum;
+        }
+#pragma unroll
+        for (int j = 0; j < COLUMNS; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int c = j * 64 + kx * 4 + e;
+                if (c >= d) continue;
+                if (p.splits > 1)
+                    p.part_o[(unit * p.splits + split) * d + c] = acc[i][j][e];
+                else
+                    static_cast<A*>(p.out)[unit * d + c] = from_float<A>(acc[i][j][e] * inv);
+            }
+    }
+}
+
+// Joins the pieces of a row's keys: a warp a (token, query head), the pieces in order.
+template <typename A>
+__global__ void __launch_bounds__(256) attention_tree_join_kernel(const TreeParams p) {
+    chain_wait();
+    const long long unit = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31, d = p.head_dim;
+    const long long token = unit / p.q_heads;
+    if (token < p.span_begin[0] || token >= min(p.span_begin[p.spans], p.tokens)) return;       // (rows of no span)
+    const float* ml = p.part_ml + unit * p.splits * 2;
+    float top = -INFINITY;
+    for (int i = lane; i < p.splits; i += 32) top = fmaxf(top, ml[2 * i]);
+    top = warp_max(top);
+    float total = 0.0f;
+    for (int i = lane; i < p.splits; i += 32) total += ml[2 * i] == -INFINITY ? 0.0f : ml[2 * i + 1] * exp2f(ml[2 * i] - top);
+    total = warp_sum(total);
+    if (p.sinks && top != -INFINITY) total += exp2f(p.sinks[unit % p.q_heads] * 1.4426950408889634f - top);
+    const float inv = top == -INFINITY ? 0.0f : 1.0f / total;
+    for (int c = lane; c < d; c += 32) {
+        float sum = 0.0f;
+        for (int i = 0; i < p.splits; ++i) {
+            const float m = ml[2 * i];
+            if (m != -INFINITY) sum = fmaf(p.part_o[(unit * p.splits + i) * d + c], exp2f(m - top), sum);
+        }
+        static_cast<A*>(p.out)[unit * d + c] = from_float<A>(sum * inv);
+    }
+}
+
+template <typename A, bool FOUR>
+static int launch_simt(const TreeParams& p, cudaStream_t stream) {
+    auto kernel = attention_tree_simt_kernel<A, 4, FOUR>;
+    int columns = 4;
+    if (p.head_dim <= 64) kernel = attention_tree_simt_kernel<A, 1, FOUR>, columns = 1;
+    else if (p.head_dim <= 128) kernel = attention_tree_simt_kernel<A, 2, FOUR>, columns = 2;
+    const size_t smem = simt_smem(p.head_dim, 64 * columns);
+    if (smem > 40 * 1024) {
+        const cudaError_t status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        CELEG_REQUIRE(status == cudaSuccess, "attention_tree: %s", cudaGetErrorString(status));
+    }
+    const int tiles = (p.max_nodes * p.group + kSimtRows - 1) / kSimtRows;
+    kernel<<<dim3(p.splits, p.kv_heads * tiles, p.spans), kSimtThreads, smem, stream>>>(p);
+    return check_launch("attention_tree");
+}
+
+template <typename A>
+static int launch_join(const TreeParams& p, cudaStream_t stream) {
+    const long long units = (long long)p.tokens * p.q_heads;
+    launch_chained(attention_tree_join_kernel<A>, dim3((unsigned)((units + 7) / 8)), dim3(256), 0, stream, p);
+    return check_launch("attention_tree (join)");
+}
+
+// Into how many pieces the keys are cut: enough for two blocks an SM, of 256 keys at least, as many as scratch holds.
+static int tree_splits(long long blocks, long long keys, long long units, int head_dim, long long scratch_elements) {
+    long long splits = 296 / (blocks > 0 ? blocks : 1);
+    if (splits > (keys + 255) / 256) splits = (keys + 255) / 256;
+    const long long room = scratch_elements / (units * (head_dim + 2));
+    if (splits > room) splits = room;
+    if (splits > 64) splits = 64;
+    return splits < 1 ? 1 : (int)splits;
+}
+
+}  // namespace celeg_b200
+
+using namespace celeg_b200;
+
+// q: [tokens, q_row_stride] with head h at columns h * head_dim; caches: one layer's [pages, kv_heads, page_tokens, head_dim],
+// page_stride elements from page to page; span_begin [spans + 1], span_context [spans], ancestors [tokens, words] (words of 32
+// bits), block_table [spans, table_stride]; out [tokens, q_heads * head_dim]. max_nodes: no span has more nodes (error 4 else);
+// max_keys: about as many keys as the longest span has, which only the number of pieces follows. scratch: float32, any number
+// of elements; the keys are cut into no more pieces than it holds.
+CELEG_API int celeg_attention_tree(const void* q, long long q_row_stride, void* out, const void* k_cache, const void* v_cache,
+                                   long long page_stride, int pages, const int* positions, const int* span_begin,
+                                   const int* span_context, const int* ancestors, int words, const int* block_table,
+                                   int table_stride, int tokens, int spans, int max_nodes, int max_keys, int q_heads,
+                                   int kv_heads, int head_dim, int page_tokens, int window, float scale, const float* sinks,
+                                   float softcap, float* scratch, long long scratch_elements, int* error_flag, int act_dtype,
+                                   cudaStream_t stream) {
+    CELEG_REQUIRE(tokens >= 0 && spans >= 0 && q_heads > 0 && kv_heads > 0 && head_dim > 0 && page_tokens > 0 && max_keys >= 0,
+                  "attention_tree: invalid sizes tokens=%d spans=%d q_heads=%d kv_heads=%d head_dim=%d page_tokens=%d", tokens,
+                  spans, q_heads, kv_heads, head_dim, page_tokens);
+    CELEG_REQUIRE(q_heads % kv_heads == 0, "attention_tree: %d query heads are not a multiple of %d kv heads", q_heads, kv_heads);
+    CELEG_REQUIRE(head_dim <= 256, "attention_tree: a head size of %d exceeds 256", head_dim);
+    CELEG_REQUIRE(max_nodes >= 1 && max_nodes <= kTreeMaxNodes && words >= (max_nodes + 31) / 32,
+                  "attention_tree: trees of up to %d nodes (at most %d) need masks of %d words, got %d", max_nodes, kTreeMaxNodes,
+                  (max_nodes + 31) / 32, words);
+    CELEG_REQUIRE(window >= 0 && softcap >= 0.0f && error_flag, "attention_tree: window %d, softcap %g, error_flag %p", window,
+                  softcap, (void*)error_flag);
+    CELEG_REQUIRE(act_dtype == kFloat32 || act_dtype == kBFloat16, "attention_tree: unknown dtype code %d", act_dtype);
+    if (tokens == 0 || spans == 0) return 0;
+    const int group = q_heads / kv_heads;
+    const long long tiles = ((long long)max_nodes * group + kSimtRows - 1) / kSimtRows;
+    CELEG_REQUIRE(spans <= 65535 && kv_heads * tiles <= 65535 && (long long)max_nodes * group <= 1 << 24,
+                  "attention_tree: %d spans of %d nodes on %d heads exceed one launch", spans, max_nodes, q_heads);
+    TreeParams p = {};
+    p.q = q;
+    p.q_row_stride = q_row_stride;
+    p.out = out;
+    p.k_cache = k_cache;
+    p.v_cache = v_cache;
+    p.page_stride = page_stride;
+    p.pages = pages;
+    p.positions = positions;
+    p.span_begin = span_begin;
+    p.span_context = span_context;
+    p.ancestors = reinterpret_cast<const unsigned*>(ancestors);
+    p.words = words;
+    p.block_table = block_table;
+    p.table_stride = table_stride;
+    p.tokens = tokens;
+    p.spans = spans;
+    p.max_nodes = max_nodes;
+    p.q_heads = q_heads;
+    p.kv_heads = kv_heads;
+    p.group = group;
+    p.head_dim = head_dim;
+    p.page_tokens = page_tokens;
+    p.window = window;
+    p.scale = scale;
+    p.sinks = sinks;
+    p.cap_in = softcap > 0.0f ? scale / softcap : 0.0f;
+    p.cap_out = softcap;
+    p.error_flag = error_flag;
+    const long long units = (long long)tokens * q_heads;
+    p.splits = tree_splits((long long)spans * kv_heads * tiles, max_keys, units, head_dim, scratch ? scratch_elements : 0);
+    p.part_o = scratch;
+    p.part_ml = scratch + units * p.splits * head_dim;
+    const size_t size = act_dtype == kFloat32 ? 4 : 2;
+    const bool four = head_dim % 4 == 0 && page_stride % 4 == 0 && q_row_stride % 4 == 0 &&
+                      (((size_t)q | (size_t)k_cache | (size_t)v_cache) & (4 * size - 1)) == 0;
+    int code;
+    if (act_dtype == kFloat32)
+        code = four ? launch_simt<float, true>(p, stream) : launch_simt<float, false>(p, stream);
+    else
+        code = four ? launch_simt<__nv_bfloat16, true>(p, stream) : launch_simt<__nv_bfloat16, false>(p, stream);
+    if (code != 0 || p.splits == 1) return code;
+    return act_dtype == kFloat32 ? launch_join<float>(p, stream) : launch_join<__nv_bfloat16>(p, stream);
+}

@@ -12,6 +12,7 @@ import functools
 from ctypes import c_float, c_int, c_longlong, c_void_p
 from typing import Optional, Tuple
 
+import numpy as np
 import torch
 
 from .csrc import build as _build
@@ -203,6 +204,16 @@ _SIGNATURES = {
     "celeg_scalar_decay_decode": [c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p,
                                   c_void_p, c_void_p, c_longlong, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p,
                                   c_void_p],
+    "celeg_attention_tree": [c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_longlong, c_int, c_void_p, c_void_p, c_void_p,
+                             c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+                             c_float, c_void_p, c_float, c_void_p, c_longlong, c_void_p, c_int, c_void_p],
+    "celeg_copy_pages": [c_void_p, c_longlong, c_longlong, c_int, c_void_p, c_longlong, c_longlong, c_int, c_int, c_int, c_int,
+                         c_int, c_int, c_void_p, c_int, c_void_p],
+    "celeg_keep_drafts": [c_void_p, c_longlong, c_longlong, c_int, c_void_p, c_longlong, c_longlong, c_int, c_int, c_int, c_int,
+                          c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
+                          c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
+    "celeg_token_logprobs": [c_void_p, c_longlong, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
+                             c_void_p],
     "celeg_moe_combine": [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
                           c_void_p],
 }
@@ -834,6 +845,201 @@ def mark_seen(seen: torch.Tensor, tokens: torch.Tensor, token_span: torch.Tensor
               count: int) -> None:
     _check(library().celeg_mark_seen(_ptr(seen), seen.shape[1], _ptr(tokens), _ptr(token_span), _ptr(span_slot),
                                      count, _stream()))
+
+
+# ------------------------------------------------------------ several continuations of a request
+TREE_MAX_NODES = 256          # drafted tokens of a request in one step
+TREE_MAX_HEAD_DIM = 256
+MAX_TOP_LOGPROBS = 128
+
+
+def _refuse(what: str) -> None:
+    raise KernelLibraryError(what)
+
+
+def _here(operator: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Every tensor on the current CUDA device, whose current stream the launch goes to."""
+    device = None
+    for tensor in tensors:
+        if tensor is None:
+            continue
+        if not tensor.is_cuda:
+            _refuse(f"{operator}: a tensor on {tensor.device}, CUDA tensors are needed")
+        if device is None:
+            device = torch._C._cuda_getDevice()
+        if tensor.get_device() != device:
+            _refuse(f"{operator}: a tensor on {tensor.device} while the current device is cuda:{device}")
+
+
+def _vector32(operator: str, tensor: torch.Tensor, elements: int, name: str, dtype: torch.dtype = torch.int32) -> None:
+    if tensor.dtype != dtype or not tensor.is_contiguous() or tensor.numel() < elements:
+        _refuse(f"{operator}: {name} must be a contiguous tensor of {dtype} with at least {elements} elements, got "
+                f"{tuple(tensor.shape)} of {tensor.dtype}, contiguous={tensor.is_contiguous()}")
+
+
+def attention_tree_scratch(device) -> torch.Tensor:
+    """Scratch of :func:`attention_tree` with room for as many pieces as it cuts the keys into at any size; one for all layers
+    of a model, or for all calls that follow one another on a stream."""
+    return torch.empty(1 << 24, dtype=torch.float32, device=device)
+
+
+def attention_tree(q: torch.Tensor, q_row_stride: int, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                   positions: torch.Tensor, span_begin: torch.Tensor, span_context: torch.Tensor, ancestors: torch.Tensor,
+                   block_table: torch.Tensor, tokens: int, spans: int, max_nodes: int, max_keys: int, q_heads: int,
+                   kv_heads: int, head_dim: int, page_tokens: int, window: Optional[int], scale: float,
+                   scratch: Optional[torch.Tensor], error_flag: torch.Tensor, sinks: Optional[torch.Tensor] = None,
+                   softcap: Optional[float] = None) -> None:
+    """Attention of drafted tokens over the paged cache (csrc/attention_tree.cuh). Span s brings the tokens
+    span_begin[s] .. span_begin[s + 1] - 1, its nodes, at most ``max_nodes`` (up to 256); its cache holds span_context[s]
+    positions and, behind them, node j at place span_context[s] + j (keys and values already stored). A node sees the cached
+    positions and the nodes whose bits its row of ``ancestors`` has (int32 [tokens, words], bit j % 32 of word j // 32; a node
+    sees itself only with its own bit), of these under a ``window`` those less than that many positions before its own:
+    ``positions`` [tokens] are the nodes' positions, a cached place's is itself. A row that sees nothing is zeros.
+    ``q`` [tokens, *] with head h at column h * head_dim, rows ``q_row_stride`` apart; ``out`` [tokens, q_heads * head_dim];
+    caches: one layer's pages. ``sinks``, ``softcap``: as for :func:`attention_generic`. ``max_keys``: about the longest span's
+    cached positions and nodes; with ``scratch`` (:func:`attention_tree_scratch`, or any float32 vector) long contexts are cut
+    into as many pieces as it has room for. Scratch is written: two launches that may run at the same time need two."""
+    name = "attention_tree"
+    dtype = q.dtype
+    code = dtype_code(dtype)
+    if k_cache.dtype != dtype or v_cache.dtype != dtype or out.dtype != dtype:
+        _refuse(f"{name}: q {dtype}, caches {k_cache.dtype} and {v_cache.dtype}, out {out.dtype}")
+    page = (kv_heads, page_tokens, head_dim)
+    inner = (page_tokens * head_dim, head_dim, 1)
+    if (k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[1:] != page or k_cache.stride()[1:] != inner
+            or v_cache.stride() != k_cache.stride()):
+        _refuse(f"{name}: caches [pages, kv_heads, page_tokens, head_dim] of pages {page} are needed, got {tuple(k_cache.shape)} and "
+                f"{tuple(v_cache.shape)} with strides {k_cache.stride()} and {v_cache.stride()}")
+    if q.dim() != 2 or q.stride(1) != 1 or q.shape[0] < tokens or q.shape[1] < q_heads * head_dim or (tokens > 1 and q.stride(0) != q_row_stride):
+        _refuse(f"{name}: q {tuple(q.shape)} with strides {q.stride()} does not hold {tokens} rows of {q_heads} x {head_dim}, {q_row_stride} apart")
+    _vector32(name, out, tokens * q_heads * head_dim, "out", dtype)
+    _vector32(name, positions, tokens, "positions")
+    _vector32(name, span_begin, spans + 1, "span_begin")
+    _vector32(name, span_context, spans, "span_context")
+    _vector32(name, error_flag, 1, "error_flag")
+    if ancestors.dim() != 2 or ancestors.shape[0] < tokens:
+        _refuse(f"{name}: ancestors {tuple(ancestors.shape)} for {tokens} tokens")
+    _vector32(name, ancestors, 0, "ancestors")
+    if block_table.dim() != 2 or block_table.shape[0] < spans or block_table.dtype != torch.int32 or block_table.stride(1) != 1:
+        _refuse(f"{name}: a block table {tuple(block_table.shape)} of {block_table.dtype} for {spans} spans")
+    if sinks is not None:
+        _vector32(name, sinks, q_heads, "sinks", torch.float32)
+    if scratch is not None:
+        _vector32(name, scratch, 0, "scratch", torch.float32)
+    _here(name, q, out, k_cache, v_cache, positions, span_begin, span_context, ancestors, block_table, error_flag, sinks, scratch)
+    _check(library().celeg_attention_tree(
+        q.data_ptr(), q_row_stride, out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0), k_cache.shape[0],
+        positions.data_ptr(), span_begin.data_ptr(), span_context.data_ptr(), ancestors.data_ptr(), ancestors.shape[1],
+        block_table.data_ptr(), block_table.stride(0), tokens, spans, max_nodes, max_keys, q_heads, kv_heads, head_dim,
+        page_tokens, int(window or 0), scale, _ptr(sinks), float(softcap or 0.0), _ptr(scratch),
+        scratch.numel() if scratch is not None else 0, error_flag.data_ptr(), code, _stream()))
+
+
+def _cache_sides(operator: str, k: torch.Tensor, v: torch.Tensor) -> tuple:
+    """What the entry points that move cached rows are given of keys and values [layers, pages, kv_heads, page_tokens, *]."""
+    if k.dim() != 5 or v.dim() != 5 or k.shape[:4] != v.shape[:4] or k.dtype != v.dtype:
+        _refuse(f"{operator}: keys and values [layers, pages, kv_heads, page_tokens, *] of one type are needed, got {tuple(k.shape)} of "
+                f"{k.dtype} and {tuple(v.shape)} of {v.dtype}")
+    layers, pages, heads, page_tokens = k.shape[:4]
+    dtype_code(k.dtype)
+    for side in (k, v):
+        dim = side.shape[4]
+        if side.numel() and side.stride()[2:] != (page_tokens * dim, dim, 1):
+            _refuse(f"{operator}: a page's heads, positions and numbers must lie side by side, got strides {side.stride()} of {tuple(side.shape)}")
+    return (k.data_ptr(), k.stride(0), k.stride(1), k.shape[4], v.data_ptr(), v.stride(0), v.stride(1), v.shape[4], layers, pages,
+            heads, page_tokens, k.element_size())
+
+
+def copy_pages(k: torch.Tensor, v: torch.Tensor, moves) -> None:
+    """Copies pages of a group of layers, keys and values in one launch (csrc/cache_pages.cu): ``moves`` is a host sequence or
+    array of (from, to, positions): the first ``positions`` of page ``to`` become those of page ``from`` in every layer, what
+    lies behind them stays. A page may be read by many moves; none may be written twice, or written by one and read by
+    another. ``k``, ``v``: [layers, pages, kv_heads, page_tokens, *]."""
+    sides = _cache_sides("copy_pages", k, v)
+    if len(moves) == 0:
+        return
+    table = np.ascontiguousarray(moves)
+    if table.ndim != 2 or table.shape[1] != 3 or table.dtype.kind not in "iu":
+        _refuse(f"copy_pages: moves are triples of whole numbers (from, to, positions), got {table.dtype} {table.shape}")
+    if table.min() < 0 or table.max() >= 1 << 31:
+        _refuse("copy_pages: a page or a number of positions is negative or too large")
+    listed = table.tolist()
+    written = {to for _, to, _ in listed}
+    if len(written) != len(listed):
+        _refuse("copy_pages: a page is written by two moves")
+    if any(source in written and source != to for source, to, _ in listed):
+        _refuse("copy_pages: a page is written by one move and read by another")
+    _here("copy_pages", k, v)
+    table = np.ascontiguousarray(table, dtype=np.int32)
+    _check(library().celeg_copy_pages(*sides, table.ctypes.data, len(listed), _stream()))
+
+
+def keep_drafts(k: torch.Tensor, v: torch.Tensor, parents: torch.Tensor, tokens: torch.Tensor, chosen: torch.Tensor,
+                span_begin: torch.Tensor, span_context: torch.Tensor, block_table: torch.Tensor, spans: int, max_nodes: int,
+                path: torch.Tensor, accepted: torch.Tensor, next_token: torch.Tensor, error_flag: torch.Tensor) -> None:
+    """What a step over drafted trees leaves behind (csrc/cache_pages.cu). Node 0 of a span is decided already; from there on the
+    path goes to the child whose token is the one ``chosen`` [tokens] after its last node (by the model: an arg-max or a draw),
+    the lowest where several are, and ends where none is. ``parents`` [tokens]: a node's parent within its span, below the node
+    itself; -1 for node 0. The path's keys and values move from places span_context[s] + path[n] to span_context[s] + n, in
+    every layer, so that they are the next cached positions. Written: ``path`` [spans, max_nodes] (-1 behind the path),
+    ``accepted`` [spans] (its length) and ``next_token`` [spans] (what was chosen after its last node). A span without nodes:
+    0 and -1. ``k``, ``v``: as for :func:`copy_pages`; a span's table row and places as for :func:`attention_tree`."""
+    name = "keep_drafts"
+    sides = _cache_sides(name, k, v)
+    count = min(parents.numel(), tokens.numel(), chosen.numel())
+    _vector32(name, parents, 0, "parents")
+    _vector32(name, tokens, 0, "tokens")
+    _vector32(name, chosen, 0, "chosen")
+    _vector32(name, span_begin, spans + 1, "span_begin")
+    _vector32(name, span_context, spans, "span_context")
+    _vector32(name, path, spans * max_nodes, "path")
+    _vector32(name, accepted, spans, "accepted")
+    _vector32(name, next_token, spans, "next_token")
+    _vector32(name, error_flag, 1, "error_flag")
+    if block_table.dim() != 2 or block_table.shape[0] < spans or block_table.dtype != torch.int32 or block_table.stride(1) != 1:
+        _refuse(f"{name}: a block table {tuple(block_table.shape)} of {block_table.dtype} for {spans} spans")
+    _here(name, k, v, parents, tokens, chosen, span_begin, span_context, block_table, path, accepted, next_token, error_flag)
+    _check(library().celeg_keep_drafts(
+        *sides, parents.data_ptr(), tokens.data_ptr(), chosen.data_ptr(), count, span_begin.data_ptr(), span_context.data_ptr(),
+        block_table.data_ptr(), block_table.stride(0), spans, max_nodes, path.data_ptr(), accepted.data_ptr(),
+        next_token.data_ptr(), error_flag.data_ptr(), _stream()))
+
+
+def token_logprobs(logits: torch.Tensor, rows: int, tokens: Optional[torch.Tensor], logprobs: Optional[torch.Tensor],
+                   entropy: Optional[torch.Tensor] = None, top_logprobs: Optional[torch.Tensor] = None,
+                   top_tokens: Optional[torch.Tensor] = None) -> None:
+    """logprobs[r] = log softmax(logits[r])[tokens[r]] in nats, ``entropy`` [rows] of the same distributions, and the
+    ``top_tokens`` [rows, k <= 128] (int32) with the largest logits, largest first, equal ones by the lower index, with their
+    log probabilities (csrc/logprobs.cu). ``logits``: float32 or bfloat16 [rows, vocab], rows at any stride; the results are
+    float32. A token outside the vocabulary has the log probability NaN; so have all of a row with a NaN, without a logit
+    above -inf or with one of +inf (a NaN counts as the smallest logit). Outputs that are None are left out."""
+    name = "token_logprobs"
+    code = dtype_code(logits.dtype)
+    if logits.dim() != 2 or logits.stride(1) != 1 or logits.shape[0] < rows or rows < 0:
+        _refuse(f"{name}: logits {tuple(logits.shape)} with strides {logits.stride()} for {rows} rows")
+    vocab = logits.shape[1]
+    if logprobs is not None:
+        if tokens is None:
+            _refuse(f"{name}: log probabilities of no tokens")
+        _vector32(name, logprobs, rows, "logprobs", torch.float32)
+        _vector32(name, tokens, rows, "tokens")
+    if entropy is not None:
+        _vector32(name, entropy, rows, "entropy", torch.float32)
+    top = 0
+    if (top_logprobs is None) != (top_tokens is None):
+        _refuse(f"{name}: top_logprobs and top_tokens come together")
+    if top_tokens is not None:
+        if top_tokens.dim() != 2 or top_logprobs.shape != top_tokens.shape:
+            _refuse(f"{name}: top_logprobs {tuple(top_logprobs.shape)} and top_tokens {tuple(top_tokens.shape)}")
+        top = top_tokens.shape[1]
+        if top > MAX_TOP_LOGPROBS or top > vocab:
+            _refuse(f"{name}: {top} alternatives, at most {MAX_TOP_LOGPROBS} and the vocabulary of {vocab}")
+        _vector32(name, top_logprobs, rows * top, "top_logprobs", torch.float32)
+        _vector32(name, top_tokens, rows * top, "top_tokens")
+    _here(name, logits, tokens, logprobs, entropy, top_logprobs, top_tokens)
+    _check(library().celeg_token_logprobs(
+        logits.data_ptr(), logits.stride(0), rows, vocab, _ptr(tokens), _ptr(logprobs), _ptr(entropy), _ptr(top_logprobs),
+        _ptr(top_tokens), top, code, _stream()))
 
 
 # ------------------------------------------------------- Dynamic Tanh blocks, matrix-state mixers
