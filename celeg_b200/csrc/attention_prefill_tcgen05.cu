@@ -89,15 +89,6 @@ struct FaParams {
 
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
 
-__device__ __forceinline__ void mbar_arrive_one(unsigned bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(bar) : "memory");
-}
-
-// The MN-major form of the instruction descriptor's B operand (bit 16): B is read as [k][n] with n contiguous.
-__host__ __device__ constexpr unsigned instruction_descriptor_b_mn(int m, int n) {
-    return instruction_descriptor(m, n) | (1u << 16);
-}
-
 template <int D>
 __global__ void __launch_bounds__(kFaThreads)
 attention_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,

@@ -5,6 +5,7 @@
 // 32 rows (node, query head of a group) of one kv head and walks its keys 64 at a time. 128 threads: for the scores a thread
 // has 4 rows x 4 keys, for the weighted sum 4 rows x 4 columns of every 64, operands from shared memory four numbers at a time.
 #include "attention_tree.cuh"
+#include "attention_tree_tcgen05.h"
 
 namespace celeg_b200 {
 
@@ -301,14 +302,18 @@ static int launch_join(const TreeParams& p, cudaStream_t stream) {
     return check_launch("attention_tree (join)");
 }
 
-// Into how many pieces the keys are cut: enough for two blocks an SM, of 256 keys at least, as many as scratch holds.
-static int tree_splits(long long blocks, long long keys, long long units, int head_dim, long long scratch_elements) {
-    long long splits = 296 / (blocks > 0 ? blocks : 1);
-    if (splits > (keys + 255) / 256) splits = (keys + 255) / 256;
+// Into how many pieces the keys are cut, as many at most as scratch holds. `problems`: (row tile, kv head, span)s, of which the
+// GPU runs `resident` at a time; `steps`: tiles of keys of the longest. A round costs its tiles and some four more for a
+// block's beginning and end; pieces have to be joined, which costs about ten and grows with their number.
+static int tree_splits(long long problems, long long resident, long long steps, long long units, int head_dim, long long scratch_elements) {
     const long long room = scratch_elements / (units * (head_dim + 2));
-    if (splits > room) splits = room;
-    if (splits > 64) splits = 64;
-    return splits < 1 ? 1 : (int)splits;
+    long long best = 1, least = 0;
+    for (long long splits = 1; splits <= 64 && splits <= steps && (splits == 1 || splits <= room); ++splits) {
+        const long long rounds = (problems * splits + resident - 1) / resident;
+        const long long cost = 4 * (rounds * ((steps + splits - 1) / splits + 4) + (splits > 1 ? 10 : 0)) + splits;
+        if (splits == 1 || cost < least) best = splits, least = cost;
+    }
+    return (int)best;
 }
 
 }  // namespace celeg_b200
@@ -373,14 +378,20 @@ CELEG_API int celeg_attention_tree(const void* q, long long q_row_stride, void* 
     p.cap_out = softcap;
     p.error_flag = error_flag;
     const long long units = (long long)tokens * q_heads;
-    p.splits = tree_splits((long long)spans * kv_heads * tiles, max_keys, units, head_dim, scratch ? scratch_elements : 0);
     p.part_o = scratch;
+    const bool tensor_cores = act_dtype == kBFloat16 && tree_tcgen05_takes(p);
+    const int tile_rows = tensor_cores ? tree_tcgen05_rows() : kSimtRows;
+    const long long reach = window > 0 && (long long)window + max_nodes < max_keys ? (long long)window + max_nodes : max_keys;
+    p.splits = tree_splits((long long)spans * kv_heads * ((max_nodes * group + tile_rows - 1) / tile_rows), 296, (reach + 63) / 64, units,
+                           head_dim, scratch ? scratch_elements : 0);
     p.part_ml = scratch + units * p.splits * head_dim;
     const size_t size = act_dtype == kFloat32 ? 4 : 2;
     const bool four = head_dim % 4 == 0 && page_stride % 4 == 0 && q_row_stride % 4 == 0 &&
                       (((size_t)q | (size_t)k_cache | (size_t)v_cache) & (4 * size - 1)) == 0;
     int code;
-    if (act_dtype == kFloat32)
+    if (tensor_cores)
+        code = launch_tree_tcgen05(p, stream);
+    else if (act_dtype == kFloat32)
         code = four ? launch_simt<float, true>(p, stream) : launch_simt<float, false>(p, stream);
     else
         code = four ? launch_simt<__nv_bfloat16, true>(p, stream) : launch_simt<__nv_bfloat16, false>(p, stream);

@@ -23,6 +23,10 @@ __device__ __forceinline__ void mbar_expect_tx(unsigned bar, unsigned bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(bytes) : "memory");
 }
 
+__device__ __forceinline__ void mbar_arrive_one(unsigned bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(bar) : "memory");
+}
+
 // Polls until the phase with the given parity has completed; false after kMaxPolls polls or two seconds,
 // whichever comes first (a try may itself block for a while, so polls alone bound nothing).
 __device__ __forceinline__ unsigned long long global_nanoseconds() {
@@ -234,6 +238,11 @@ __host__ __device__ constexpr unsigned instruction_descriptor(int m, int n) {
     return (1u << 4) | (1u << 7) | (1u << 10) | ((unsigned)(n >> 3) << 17) | ((unsigned)(m >> 4) << 24);
 }
 
+
+// The MN-major form of the instruction descriptor's B operand (bit 16): B is read as [k][n] with n contiguous.
+__host__ __device__ constexpr unsigned instruction_descriptor_b_mn(int m, int n) {
+    return instruction_descriptor(m, n) | (1u << 16);
+}
 
 // Host: the tensor map of a [rows, cols] bfloat16 matrix with `ld` elements between rows, read in boxes
 // of box_rows x 64 elements with the 128-byte swizzle (cached per matrix). False with the reason in
