@@ -302,15 +302,16 @@ static int launch_join(const TreeParams& p, cudaStream_t stream) {
     return check_launch("attention_tree (join)");
 }
 
-// Into how many pieces the keys are cut, as many at most as scratch holds. `problems`: (row tile, kv head, span)s, of which the
-// GPU runs `resident` at a time; `steps`: tiles of keys of the longest. A round costs its tiles and some four more for a
-// block's beginning and end; pieces have to be joined, which costs about ten and grows with their number.
-static int tree_splits(long long problems, long long resident, long long steps, long long units, int head_dim, long long scratch_elements) {
-    const long long room = scratch_elements / (units * (head_dim + 2));
+// Into how many pieces the keys are cut. `problems`: (row tile, kv head, span)s; `steps`: tiles of keys of the longest. A round
+// of blocks costs its tiles and some `ends` more for a block's beginning and end. Up to `cluster` pieces meet in a cluster,
+// which costs little, but a cluster wants neighbouring SMs; more pieces, as many as scratch holds, want a second launch.
+static int tree_splits(long long problems, const TreeTile& tile, long long steps, long long room) {
     long long best = 1, least = 0;
-    for (long long splits = 1; splits <= 64 && splits <= steps && (splits == 1 || splits <= room); ++splits) {
-        const long long rounds = (problems * splits + resident - 1) / resident;
-        const long long cost = 4 * (rounds * ((steps + splits - 1) / splits + 4) + (splits > 1 ? 10 : 0)) + splits;
+    for (long long splits = 1; splits <= 64 && splits <= steps && (splits <= tile.cluster || splits <= room); ++splits) {
+        const long long at_once = splits <= tile.cluster ? tile.problems_at_once[splits] : 0;
+        const long long rounds = at_once > 0 ? (problems + at_once - 1) / at_once : (problems * splits + tile.blocks - 1) / tile.blocks;
+        const long long joining = splits == 1 ? 0 : splits <= tile.cluster ? 4 : 8;
+        const long long cost = 4 * (rounds * ((steps + splits - 1) / splits + tile.ends) + joining) + splits;
         if (splits == 1 || cost < least) best = splits, least = cost;
     }
     return (int)best;
@@ -372,6 +373,9 @@ CELEG_API int celeg_attention_tree(const void* q, long long q_row_stride, void* 
     p.head_dim = head_dim;
     p.page_tokens = page_tokens;
     p.window = window;
+    p.page_shift = -1;
+    for (int shift = 0; shift < 31; ++shift)
+        if (page_tokens == 1 << shift) p.page_shift = shift;
     p.scale = scale;
     p.sinks = sinks;
     p.cap_in = softcap > 0.0f ? scale / softcap : 0.0f;
@@ -380,11 +384,13 @@ CELEG_API int celeg_attention_tree(const void* q, long long q_row_stride, void* 
     const long long units = (long long)tokens * q_heads;
     p.part_o = scratch;
     const bool tensor_cores = act_dtype == kBFloat16 && tree_tcgen05_takes(p);
-    const int tile_rows = tensor_cores ? tree_tcgen05_rows() : kSimtRows;
+    TreeTile tile = {kSimtRows, 296, 4, 1, {0}};
+    if (tensor_cores) tile = tree_tcgen05_tile(p);
     const long long reach = window > 0 && (long long)window + max_nodes < max_keys ? (long long)window + max_nodes : max_keys;
-    p.splits = tree_splits((long long)spans * kv_heads * ((max_nodes * group + tile_rows - 1) / tile_rows), 296, (reach + 63) / 64, units,
-                           head_dim, scratch ? scratch_elements : 0);
-    p.part_ml = scratch + units * p.splits * head_dim;
+    p.splits = tree_splits((long long)spans * kv_heads * ((max_nodes * group + tile.rows - 1) / tile.rows), tile, (reach + 63) / 64,
+                           scratch ? scratch_elements / (units * (head_dim + 2)) : 0);
+    if (p.splits <= tile.cluster) p.part_o = nullptr;
+    p.part_ml = p.part_o ? scratch + units * p.splits * head_dim : nullptr;
     const size_t size = act_dtype == kFloat32 ? 4 : 2;
     const bool four = head_dim % 4 == 0 && page_stride % 4 == 0 && q_row_stride % 4 == 0 &&
                       (((size_t)q | (size_t)k_cache | (size_t)v_cache) & (4 * size - 1)) == 0;
@@ -395,6 +401,6 @@ CELEG_API int celeg_attention_tree(const void* q, long long q_row_stride, void* 
         code = four ? launch_simt<float, true>(p, stream) : launch_simt<float, false>(p, stream);
     else
         code = four ? launch_simt<__nv_bfloat16, true>(p, stream) : launch_simt<__nv_bfloat16, false>(p, stream);
-    if (code != 0 || p.splits == 1) return code;
+    if (code != 0 || !p.part_o) return code;
     return act_dtype == kFloat32 ? launch_join<float>(p, stream) : launch_join<__nv_bfloat16>(p, stream);
 }

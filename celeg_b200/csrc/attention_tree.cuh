@@ -30,6 +30,7 @@ struct TreeParams {
     const int* block_table;        // [spans, table_stride]
     int words, table_stride, pages, tokens, spans, max_nodes;
     int q_heads, kv_heads, group, head_dim, page_tokens, window, splits;
+    int page_shift;                // page_tokens = 1 << page_shift, -1: no power of two
     float scale;
     const float* sinks;            // [q_heads] or null
     float cap_in, cap_out;         // capped scores: cap_out tanh(cap_in * raw score), scale / cap and cap; 0: none

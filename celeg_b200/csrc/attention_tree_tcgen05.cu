@@ -1,50 +1,95 @@
-// Attention of a tree of drafted tokens over the paged cache on the fifth-generation tensor cores, bfloat16, head sizes D of 64
-// and 128, pages of 8, 16, 32 or 64 positions that lie side by side (see attention_tree.cuh for the operator):
+// Attention of a tree of drafted tokens over the paged cache on the fifth-generation tensor cores: bfloat16, head sizes that are
+// multiples of 8 up to 128, pages of any size (see attention_tree.cuh for the operator).
 //
-//   grid = (row tiles x pieces of the keys, kv heads, spans). A row tile is 128 rows (node, query head of the group) of one kv
-//   head, so that a key is read once for a whole group and tree; the pieces are of whole blocks of 64 keys.
-//   Six warps. Warp 0 brings a block's K and V page by page through the block table by TMA (128-byte swizzle, a lane a copy,
-//   pages looked up a block ahead) into a ring of stages; warp 1 issues S = Q K^T and O += P V (tcgen05.mma, P from tensor
-//   memory, V as it lies in the cache); warps 2 to 5 are the softmax, a thread a row. S and P exist twice, so that the products
-//   of one block run while the softmax is busy with the next. Two blocks an SM (81 or 97 KiB of shared memory, 256 columns of
-//   tensor memory) hide one another's waits.
-//   The rows of Q are gathered by the softmax threads themselves (a head here, a node there) and written in the layout that
-//   TMA gives the keys.
+//   grid = (row tiles x pieces of the keys, kv heads, spans). A row is a (node, query head of the group) of one kv head, so that
+//   a key is read once for a whole group and tree; keys come in blocks of 64, a piece is a run of whole blocks.
+//   Fourteen warps, one block an SM. Two teams, each of a warp that issues its products (tcgen05.mma: S = Q K^T, and O += P V
+//   with P from tensor memory and V as it lies in the cache) and four warps of softmax, a thread a row. A row tile has 128
+//   rows and the teams take its even and odd blocks of keys, with outputs, maxima and sums of their own; or, where there are
+//   more rows, 256 rows, a team 128 of them, and every block of keys serves both teams. A team's S and P exist twice, so that its
+//   products run while its softmax is busy with another block. A step of the softmax is a chain of waits around its
+//   exponentials, which the two teams hide from one another.
+//   Four warps copy K and V: rows of 16-byte pieces by cp.async, written in the layout with the 128-byte swizzle that the
+//   products want. (By TMA, a box a page, a page of 16 positions x 64 took 110 cycles whoever asked for it, 880 cycles for a
+//   block of 16 KiB of K and V; these copies take 320, and at 6.9 TB/s the memory gives an SM a block in 660.) What holds no key
+//   of the span arrives as zeros.
+//   At the end the teams' results meet in shared memory, and those of up to eight pieces of the keys, which are a cluster, in
+//   one another's; more pieces go through scratch and a second launch.
 //
 // Blocks of keys before the tree are seen whole by every row and need no mask. In the others a row's mask is 64 bits, cut from
-// its words of ancestors; values that no row sees are overwritten with zeros, and a value that is not finite is taken out and
-// added to the rows that do see it at the end (a weight of zero times it would reach the others).
+// its words of ancestors; a value that is not finite is taken out there and added to the rows that do see it at the end (a weight
+// of zero times it would reach the others).
 //
-// The weights are rounded to bfloat16 for their product with V; the denominator adds up the rounded ones, so that the outputs
-// are exact averages of what was multiplied. Rows beyond the span's and warps without rows take no exponentials.
+// The weights are rounded to bfloat16 for their product with V (the denominator adds them up before): 2^-9 of each, at random.
+// Warps without rows take no exponentials.
 #include "attention_tree.cuh"
 #include "attention_tree_tcgen05.h"
-#include "ring_drain.h"
 #include "tcgen05.cuh"
+
+#include <atomic>
 
 namespace celeg_b200 {
 
-constexpr int kTtThreads = 192;
-constexpr int kTtM = 128;                 // rows per tile
+constexpr int kTtCopyWarps = 4;           // a pair of them brings every other block
+constexpr int kTtSoftmaxFirst = kTtCopyWarps + 2;
+constexpr int kTtThreads = 32 * (kTtSoftmaxFirst + 8);
+constexpr int kTtM = 128;                 // rows of a team
 constexpr int kTtN = 64;                  // keys per block
+constexpr int kTtMaxCluster = 8;          // pieces of the keys that meet in shared memory
+constexpr unsigned kTtTmemColumns = 512;
 
-template <int D>
+// D: the head size padded to 64 or 128. Rows of 128 lie in shared memory as two halves of 64 (a swizzled row is 128 bytes).
+template <int D, bool PAIRED>
 struct TtLayout {
     static constexpr int kHalves = D / 64;
-    static constexpr int kStages = D == 64 ? 4 : 2;
     static constexpr unsigned kQHalf = kTtM * 128, kKvHalf = kTtN * 128;
-    static constexpr unsigned kQBytes = kHalves * kQHalf;       // 16 or 32 KiB
+    static constexpr unsigned kQBytes = kHalves * kQHalf;       // 16 or 32 KiB a team
     static constexpr unsigned kKvBytes = kHalves * kKvHalf;     // 8 or 16 KiB each for a block's K and V
-    static constexpr unsigned kSmemBytes = kQBytes + kStages * 2 * kKvBytes + 1024;
-    // Tensor memory: S of even and odd blocks at columns 0 and 64, O from 128 on; P behind O at a head size of 64, over the
-    // scores it is made of at 128.
-    static constexpr unsigned kOColumn = 2 * kTtN;
+    static constexpr int kStages = D == 64 ? 12 : PAIRED ? 5 : 6;
+    static constexpr unsigned kAllQ = PAIRED ? 2 * kQBytes : kQBytes;
+    static constexpr unsigned kSmemBytes = kAllQ + kStages * 2 * kKvBytes + 1024;      // 209 to 225 KiB
+    // what meets at the end lies where queries and keys were: rows of results (16-byte pieces of eight rows in different banks),
+    // 2 x 128 and one more of every part, their maxima and sums, the rows' (token, query head) numbers
+    static constexpr int kPitch = D + 4, kMeetRows = 2 * kTtM + 2 * kTtMaxCluster;
+    static constexpr unsigned kStatsAt = kMeetRows * kPitch * 4, kUnitsAt = kStatsAt + kMeetRows * 8;
+    static_assert(kUnitsAt + 2 * kTtM * 4 + 1024 <= kSmemBytes, "the results meet where queries and keys were");
+    // Tensor memory of a team: scores of its even and odd blocks at columns 0 and 64, O from 128 on, the weights behind O at a
+    // head size of 64 and over the scores they were made of at 128.
+    static constexpr unsigned kTeamColumns = 256, kOColumn = 2 * kTtN;
     static constexpr bool kOverScores = D == 128;
-    static __device__ __forceinline__ unsigned p_column(int i) {
-        return kOverScores ? (unsigned)((i & 1) * kTtN) : 2 * kTtN + D + (unsigned)((i & 1) * (kTtN / 2));
+    static __device__ __forceinline__ unsigned p_column(int n) {
+        return kOverScores ? (unsigned)((n & 1) * kTtN) : 2 * kTtN + D + (unsigned)((n & 1) * (kTtN / 2));
     }
 };
-constexpr unsigned kTtTmemColumns = 256;
+
+__device__ __forceinline__ unsigned pack_bf16_pair(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const unsigned*>(&v);
+}
+
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+// The place that `address` is in block `rank`'s shared memory, or in this block's own.
+__device__ __forceinline__ unsigned peer_address(unsigned address, unsigned rank, bool other) {
+    unsigned peer;
+    if (other)
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(peer) : "r"(address), "r"(rank));
+    else
+        asm volatile("{\n\t.reg .u32 own;\n\tmov.u32 own, %%cluster_ctarank;\n\tmapa.shared::cluster.u32 %0, %1, own;\n\t}\n" : "=r"(peer) : "r"(address));
+    return peer;
+}
+__device__ __forceinline__ void store_2(unsigned peer, float a, float b) {
+    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};\n" ::"r"(peer), "f"(a), "f"(b) : "memory");
+}
+__device__ __forceinline__ void store_4(unsigned peer, unsigned a, unsigned b, unsigned c, unsigned d) {
+    asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(peer), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ float fast_exp2(float x) {
+    float e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x));
+    return e;
+}
 
 // The keys key_base .. key_base + 63 that a row sees, a bit each.
 __device__ __forceinline__ unsigned long long tree_visible(const TreeParams& p, const TreeSpan& s, const unsigned* mask, int position,
@@ -81,54 +126,95 @@ __device__ __forceinline__ unsigned long long tree_visible(const TreeParams& p, 
 
 __device__ __forceinline__ bool not_finite(unsigned bf16_bits) { return (bf16_bits & 0x7f80u) == 0x7f80u; }
 
-template <int D>
-__global__ void __launch_bounds__(kTtThreads)
-attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const TreeParams p) {
+// 32 scores of a row to their weights relative to `base` (scores times `to_log2`), packed in pairs of bfloat16; returns the sum
+// of the weights and takes the largest score along.
+__device__ __forceinline__ float tree_weights(const float* sc, unsigned long long scale2, unsigned long long neg_base2, unsigned (&packed)[16],
+                                              float& largest) {
+    unsigned long long sums[4] = {0ull, 0ull, 0ull, 0ull};      // (0.0f, 0.0f) each
+    float tops[2] = {largest, largest};
+#pragma unroll
+    for (int j2 = 0; j2 < 16; ++j2) {
+        float x0, x1, a, b;
+        tops[j2 & 1] = max3_f32(tops[j2 & 1], sc[2 * j2], sc[2 * j2 + 1]);
+        unpack_f32x2(fma_f32x2(pack_f32x2(sc[2 * j2], sc[2 * j2 + 1]), scale2, neg_base2), x0, x1);
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(x0));
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(b) : "f"(x1));
+        sums[j2 & 3] = add_f32x2(sums[j2 & 3], pack_f32x2(a, b));
+        packed[j2] = pack_bf16_pair(a, b);                      // (key 2 j2 in the lower half)
+    }
+    largest = fmaxf(tops[0], tops[1]);
+    float s0, s1;
+    unpack_f32x2(add_f32x2(add_f32x2(sums[0], sums[1]), add_f32x2(sums[2], sums[3])), s0, s1);
+    return s0 + s1;
+}
+
+// PAIRED: row tiles of 256 rows, a team a half of them, every block of keys for both; otherwise of 128 rows, a team every other block.
+template <int D, bool PAIRED>
+__global__ void __launch_bounds__(kTtThreads, 1) attention_tree_tcgen05_kernel(const TreeParams p) {
     extern __shared__ __align__(1024) unsigned char smem_raw[];
-    using L = TtLayout<D>;
-    constexpr int kStages = L::kStages;
-    __shared__ __align__(8) unsigned long long kv_full[kStages], kv_empty[kStages], q_full, s_full[2], p_full[2], o_full[2];
+    using L = TtLayout<D, PAIRED>;
+    constexpr int kStages = L::kStages, kTileRows = PAIRED ? 2 * kTtM : kTtM;
+    __shared__ __align__(8) unsigned long long kv_full[kStages], kv_empty[kStages], q_full[2], s_full[2][2], p_full[2][2], o_full[2][2];
     __shared__ unsigned tmem_base_slot;
     __shared__ int lowest_s, highest_s, bad_values;
 
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    // (the warp's number comes from a shuffle so that what follows from it is known to be the same in all lanes: descriptors and
+    // addresses of the products are then made once, in uniform registers)
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const int span = blockIdx.z, kvh = blockIdx.y;
-    const int tiles = (p.max_nodes * p.group + kTtM - 1) / kTtM;
-    const int row0 = (blockIdx.x % tiles) * kTtM, split = blockIdx.x / tiles;
-    const TreeSpan s = tree_span(p, span);
-    const int rows = min(s.nodes * p.group - row0, kTtM);
-    if (rows <= 0) return;                                      // (the whole block, before anything is taken)
-
+    const int row0 = (blockIdx.x / p.splits) * kTileRows, split = blockIdx.x % p.splits;
     if (tid == 0) {
         for (int i = 0; i < kStages; ++i) {
-            mbar_init(smem_u32(&kv_full[i]), 1);
-            mbar_init(smem_u32(&kv_empty[i]), 1);
+            mbar_init(smem_u32(&kv_full[i]), 64);
+            mbar_init(smem_u32(&kv_empty[i]), PAIRED ? 2 : 1);
         }
-        mbar_init(smem_u32(&q_full), 128);
-        for (int b = 0; b < 2; ++b) {
-            mbar_init(smem_u32(&s_full[b]), 1);
-            mbar_init(smem_u32(&p_full[b]), 128);
-            mbar_init(smem_u32(&o_full[b]), 1);
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(smem_u32(&q_full[t]), 128);
+            for (int b = 0; b < 2; ++b) {
+                mbar_init(smem_u32(&s_full[t][b]), 1);
+                mbar_init(smem_u32(&p_full[t][b]), 128);
+                mbar_init(smem_u32(&o_full[t][b]), 1);
+            }
         }
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
         lowest_s = 0x7fffffff;
         highest_s = -0x7fffffff - 1;
         bad_values = 0;
     }
-    if (warp == 0) tmem_alloc(smem_u32(&tmem_base_slot), kTtTmemColumns);
+    if (warp == kTtCopyWarps) tmem_alloc(smem_u32(&tmem_base_slot), kTtTmemColumns);
+    chain_release();
+    chain_wait();                                               // (what comes before this line may run under the kernel before)
+    const TreeSpan s = tree_span(p, span);
+    const int rows = min(s.nodes * p.group - row0, kTileRows);  // (of a whole cluster alike)
+    const int d = p.head_dim;
+
+    const bool softmax = warp >= kTtSoftmaxFirst;
+    const int team = softmax ? (warp - kTtSoftmaxFirst) >> 2 : warp < kTtCopyWarps ? warp >> 1 : warp - kTtCopyWarps;
+    // a softmax thread's row; a warp may touch the 32 lanes of tensor memory that its number gives
+    const int lane_row = (warp & 3) * 32 + lane, row = lane_row + (PAIRED ? team * kTtM : 0);
+    const bool live = softmax && row < rows;
+    const int node = rows > 0 ? s.begin + (row0 + min(row, rows - 1)) / p.group : 0;
+    const int head = rows > 0 ? kvh * p.group + (row0 + min(row, rows - 1)) % p.group : 0;
+    constexpr int kQueryPieces = PAIRED ? D / 8 : D / 16;       // 16-byte pieces of its query a thread brings: a row, or half of one
+    uint4 query[kQueryPieces];                                  // (under way while the block sets up)
+    if (softmax) {
+        const uint4* q = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.q) + (size_t)node * p.q_row_stride + (size_t)head * d);
+#pragma unroll
+        for (int c0 = 0; c0 < kQueryPieces; ++c0) {
+            const int c = PAIRED ? c0 : team * kQueryPieces + c0;
+            query[c0] = live && 8 * c < d ? __ldg(q + c) : make_uint4(0u, 0u, 0u, 0u);
+        }
+    }
+    const int position = p.window && rows > 0 ? p.positions[node] : 0;
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
     const unsigned tmem_base = tmem_base_slot;
-
-    // a softmax thread's row
-    const int row = (warp & 3) * 32 + lane;                     // (of warps 2 to 5: the TMEM lane)
-    const bool live = warp >= 2 && row < rows;
-    const int node = s.begin + (row0 + min(row, rows - 1)) / p.group;
-    const int head = kvh * p.group + (row0 + min(row, rows - 1)) % p.group;
-    int position = 0;
+    if (rows <= 0) {
+        if (warp == kTtCopyWarps) tmem_dealloc(tmem_base, kTtTmemColumns);
+        return;
+    }
     if (p.window) {
-        position = p.positions[node];
         if (live) {
             atomicMin(&lowest_s, position);
             atomicMax(&highest_s, position);
@@ -143,154 +229,229 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
     const int per_split = (all_end - all_begin + p.splits - 1) / p.splits;
     const int block_begin = all_begin + split * per_split;
     const int blocks = max(0, min(per_split, all_end - block_begin));
+    // the team's n-th block is the piece's block kStride n + kFirst
+    constexpr int kStride = PAIRED ? 1 : 2;
+    const int first_block = PAIRED ? 0 : team;
+    const int mine = PAIRED ? blocks : (blocks + 1 - team) / 2;
+    const bool idle = PAIRED && team * kTtM >= rows;            // (a team without rows still gives its share of the stages back)
 
     const unsigned smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    const unsigned q_addr = smem_base;
-    const unsigned k_addr = q_addr + L::kQBytes, v_addr = k_addr + kStages * L::kKvBytes;
+    const unsigned q_addr = smem_base + (PAIRED ? team * L::kQBytes : 0);
+    const unsigned k_addr = smem_base + L::kAllQ, v_addr = k_addr + kStages * L::kKvBytes;
+    const unsigned* mask = p.ancestors + (size_t)node * p.words;
+    const unsigned team_base = tmem_base + (unsigned)team * L::kTeamColumns;
+    const unsigned row_base = team_base + ((unsigned)((warp & 3) * 32) << 16);
 
     int error = 0;
-    if (warp == 0) {
-        // ------------------------------------------------------------------------------------ producer
+    float used_max = -INFINITY, run_sum = 0.0f;
+    auto wait = [&](unsigned long long& bar, int parity) {
+        return __all_sync(0xffffffffu, mbar_wait(smem_u32(&bar), (unsigned)parity)) != 0;
+    };
+    if (warp < kTtCopyWarps) {
+        // ------------------------------------------------------------------------------ K and V, block by block
+        // A pair of warps brings every other block: a thread has one 16-byte piece of every eighth row of K and of V.
+        const int pair = warp >> 1, thread = tid & 63;
+        const int piece = thread & 7, row_in_8 = thread >> 3;
+        const unsigned to = (unsigned)row_in_8 * 128u + (unsigned)((piece ^ row_in_8) << 4);
         const int* table = p.block_table + (size_t)span * p.table_stride;
-        const int pages_per_block = kTtN / p.page_tokens;                          // 1 to 8
-        const int pieces = 2 * L::kHalves * pages_per_block;                       // K and V, halves of a row
-        static_assert(2 * L::kHalves * 8 <= 32, "a lane brings one piece");
-        auto lookup = [&](int kb, int piece) -> int {
-            const int key0 = kb * kTtN + (piece / (2 * L::kHalves)) * p.page_tokens;
-            if (piece >= pieces || kb >= block_begin + blocks || key0 > last_key || key0 + p.page_tokens <= first_key) return 0;
-            const int logical = key0 / p.page_tokens;
-            const int page = logical < p.table_stride ? table[logical] : -1;
-            if (page < 0 || page >= p.pages) {
-                atomicExch(p.error_flag, 2);
-                return 0;                                                          // (keys nobody may see, or reported: any page will do)
-            }
-            return page;
-        };
-        int page = lookup(block_begin, lane);
-        int brought = 0;
+        const __nv_bfloat16* k = static_cast<const __nv_bfloat16*>(p.k_cache) + piece * 8 + (size_t)kvh * p.page_tokens * d;
+        const __nv_bfloat16* v = static_cast<const __nv_bfloat16*>(p.v_cache) + piece * 8 + (size_t)kvh * p.page_tokens * d;
         bool ok = true;
-        for (int i = 0; i < blocks && ok; ++i) {
-            const int mine = page;
-            page = lookup(block_begin + i + 1, lane);
-            const int stage = i % kStages;
-            const unsigned bar = smem_u32(&kv_full[stage]);
-            int got = 1;
-            if (lane == 0) {
-                if (i >= kStages && !mbar_wait_suspended(smem_u32(&kv_empty[stage]), ((i / kStages) - 1) & 1)) got = 0;
-                if (got) mbar_expect_tx(bar, 2 * L::kKvBytes);
+        auto begin_block = [&](int i) {                         // its stage is free
+            return i < kStages || wait(kv_empty[i % kStages], ((i / kStages) - 1) & 1);
+        };
+        auto end_block = [&](int i) {                           // the barrier counts this thread when its copies so far have landed
+            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];\n" ::"r"(smem_u32(&kv_full[i % kStages])) : "memory");
+        };
+        // one piece of a row of K and of V (of both halves of it), or zeros
+        auto copy = [&](unsigned k_to, unsigned v_to, const __nv_bfloat16* k_from, const __nv_bfloat16* v_from, bool there) {
+#pragma unroll
+            for (int half = 0; half < L::kHalves; ++half) {
+                const bool some = there && half * 64 + piece * 8 < d;
+                const unsigned bytes = some ? 16 : 0;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(k_to + half * L::kKvHalf), "l"(some ? k_from + half * 64 : k), "r"(bytes) : "memory");
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(v_to + half * L::kKvHalf), "l"(some ? v_from + half * 64 : v), "r"(bytes) : "memory");
             }
-            ok = __shfl_sync(0xffffffffu, got, 0) != 0;
-            if (ok && lane < pieces) {
-                const int pg = lane / (2 * L::kHalves), side = lane % 2, half = (lane / 2) % L::kHalves;
-                const unsigned to = (side ? v_addr : k_addr) + stage * L::kKvBytes + half * L::kKvHalf + pg * (unsigned)p.page_tokens * 128u;
-                tma_load_2d(to, side ? &map_v : &map_k, bar, half * 64, (mine * p.kv_heads + kvh) * p.page_tokens);
+        };
+        if (p.page_shift >= 3) {
+            // Pages of a power of two positions, eight at least: eight rows of a block are consecutive in a page. The table is
+            // read 32 entries at a time, a lane each, and a round ahead: an entry a block would be a round trip to the L2 a
+            // block. (With an address of its own for every row the instructions of the copies were what bounded the kernel.)
+            const int first_page = block_begin * kTtN >> p.page_shift, last_page = last_key >> p.page_shift, in_page = p.page_tokens - 1;
+            auto entries = [&](int round) -> int {
+                const int logical = first_page + round * 32 + lane;
+                return logical <= last_page && logical < p.table_stride ? table[logical] : -1;
+            };
+            const unsigned stride = (unsigned)p.page_stride;    // (fits: see tree_tcgen05_takes)
+            int held = entries(0), ahead = entries(1), round = 0;
+            for (int i = pair; i < blocks; i += 2) {
+                const int key_base = (block_begin + i) * kTtN, index = (key_base >> p.page_shift) - first_page;
+                if (index >> 5 != round) {
+                    held = ahead;
+                    ahead = entries(++round + 1);
+                }
+                ok = begin_block(i);
+                if (!ok) break;
+                const unsigned stage_at = (unsigned)(i % kStages) * L::kKvBytes + to, k_to = k_addr + stage_at, v_to = v_addr + stage_at;
+                const int pages = max(1, kTtN >> p.page_shift);
+                const bool good = (unsigned)(lane - (index & 31)) >= (unsigned)pages || (unsigned)held < (unsigned)p.pages;
+                if (__all_sync(0xffffffffu, good) && key_base >= first_key && key_base + kTtN - 1 <= last_key) {
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) {
+                        const unsigned page = (unsigned)__shfl_sync(0xffffffffu, held, index + (u * 8 >> p.page_shift));
+                        const size_t offset = (size_t)page * stride + (unsigned)((((key_base + u * 8) & in_page) + row_in_8) * d);
+                        copy(k_to + u * 1024u, v_to + u * 1024u, k + offset, v + offset, true);
+                    }
+                } else {
+                    for (int u = 0; u < 8; ++u) {
+                        const int key = key_base + u * 8 + row_in_8;
+                        const int page = __shfl_sync(0xffffffffu, held, index + (u * 8 >> p.page_shift));
+                        const bool wanted = key >= first_key && key <= last_key, there = wanted && (unsigned)page < (unsigned)p.pages;
+                        if (wanted && !there) atomicExch(p.error_flag, 2);
+                        const size_t offset = there ? (size_t)(unsigned)page * stride + (unsigned)((key & in_page) * d) : 0;
+                        copy(k_to + u * 1024u, v_to + u * 1024u, k + offset, v + offset, there);
+                    }
+                }
+                end_block(i);
             }
-            brought += ok;
+        } else {
+            // any other pages: a lane looks up two of a block's 64 keys, a block of its pair ahead
+            auto look_up = [&](int i, int u) -> int {
+                const int key = (block_begin + i) * kTtN + u * 32 + lane;
+                if (i >= blocks || key < first_key || key > last_key) return -2;
+                const int logical = key / p.page_tokens;
+                return logical < p.table_stride ? table[logical] : -1;
+            };
+            int page[2] = {look_up(pair, 0), look_up(pair, 1)};
+            for (int i = pair; i < blocks; i += 2) {
+                long long offsets[2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int key = (block_begin + i) * kTtN + u * 32 + lane;
+                    offsets[u] = -1;
+                    if (page[u] >= 0 && page[u] < p.pages) offsets[u] = (long long)page[u] * p.page_stride + (long long)(key % p.page_tokens) * d;
+                    else if (page[u] != -2) atomicExch(p.error_flag, 2);
+                    page[u] = look_up(i + 2, u);
+                }
+                ok = begin_block(i);
+                if (!ok) break;
+                const unsigned stage_at = (unsigned)(i % kStages) * L::kKvBytes + to;
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    const long long offset = __shfl_sync(0xffffffffu, offsets[u >> 2], (u & 3) * 8 + row_in_8);
+                    const long long from = offset >= 0 ? offset : 0;
+                    copy(k_addr + stage_at + u * 1024u, v_addr + stage_at + u * 1024u, k + from, v + from, offset >= 0);
+                }
+                end_block(i);
+            }
         }
-        if (lane == 0) {
-            if (!ok) error = 61;
-            // whichever role gives up: the block does not end before its copies have landed
-            drain_ring(max(0, brought - kStages), brought, kStages,
-                       [&](int stage, unsigned parity) { mbar_wait_suspended(smem_u32(&kv_full[stage]), parity); });
-        }
-    } else if (warp == 1) {
-        // ---------------------------------------------------------------------------------- MMA issuer
+        asm volatile("cp.async.wait_all;\n" ::: "memory");
+        if (!ok) error = 61;
+    } else if (!softmax) {
+        // ------------------------------------------------------------------------------------ a team's products
+        // The whole warp waits, one elected lane issues.
         constexpr unsigned idesc_s = instruction_descriptor(kTtM, kTtN);
         constexpr unsigned idesc_o = instruction_descriptor_b_mn(kTtM, 64);        // (64 columns of O at a time)
         const unsigned long long desc_q = smem_descriptor(q_addr);
-        auto wait = [&](unsigned long long& bar, int parity) {
-            return __all_sync(0xffffffffu, mbar_wait_suspended(smem_u32(&bar), (unsigned)parity)) != 0;
-        };
-        auto scores = [&](int i) -> bool {
-            const int stage = i % kStages;
+        // S of the team's n-th block, as soon as its keys are there. (The softmax has read the buffer's last content: P of block
+        // n - 1 was complete before this point. Where P lies over the scores, its product must be done as well.)
+        auto scores = [&](int n) -> bool {
+            const int i = kStride * n + first_block, stage = i % kStages;
             if (!wait(kv_full[stage], (i / kStages) & 1)) return false;
-            if (L::kOverScores && i >= 2 && !wait(o_full[i & 1], ((i - 2) >> 1) & 1)) return false;
+            if (L::kOverScores && n >= 2 && !wait(o_full[team][n & 1], ((n - 2) >> 1) & 1)) return false;
+            // (the copies wrote through the generic proxy, the products read through the asynchronous one)
+            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
             tcgen05_fence_after();
             const unsigned long long desc_k = smem_descriptor(k_addr + stage * L::kKvBytes);
             if (elect_one()) {
 #pragma unroll
                 for (int kk = 0; kk < D / kUmmaK; ++kk) {
                     const unsigned long long half = kk >> 2, part = 2 * (kk & 3);
-                    umma_bf16(tmem_base + (unsigned)((i & 1) * kTtN), desc_q + half * (L::kQHalf >> 4) + part,
+                    umma_bf16(team_base + (unsigned)((n & 1) * kTtN), desc_q + half * (L::kQHalf >> 4) + part,
                               desc_k + half * (L::kKvHalf >> 4) + part, idesc_s, kk > 0 ? 1u : 0u);
                 }
-                umma_commit(smem_u32(&s_full[i & 1]));
+                umma_commit(smem_u32(&s_full[team][n & 1]));
             }
             __syncwarp();
             return true;
         };
-        if (blocks > 0) {
-            if (!wait(q_full, 0)) error = 62;
-            if (!error && !scores(0)) error = 63;
-        }
-        for (int i = 0; i < blocks && !error; ++i) {
-            // (the scores of the next block: the softmax has read that buffer, P of block i - 1 was complete before this point)
-            if (i + 1 < blocks && !scores(i + 1)) {
-                error = 63;
-                break;
-            }
-            const int stage = i % kStages;
-            if (!wait(p_full[i & 1], (i >> 1) & 1)) {
-                error = 64;
-                break;
-            }
-            tcgen05_fence_after();
-            const unsigned long long desc_v = smem_descriptor(v_addr + stage * L::kKvBytes);
-            if (elect_one()) {
-#pragma unroll
-                for (int kk = 0; kk < kTtN / kUmmaK; ++kk) {
-#pragma unroll
-                    for (int half = 0; half < L::kHalves; ++half)
-                        umma_bf16_a_tmem(tmem_base + L::kOColumn + half * 64, tmem_base + L::p_column(i) + (unsigned)(kk * 8),
-                                         desc_v + (unsigned long long)(half * (L::kKvHalf >> 4) + kk * 128), idesc_o, (i > 0 || kk > 0) ? 1u : 0u);
+        if (idle) {
+            for (int n = 0; n < mine; ++n) {
+                if (!wait(kv_full[n % kStages], (n / kStages) & 1)) {
+                    error = 63;
+                    break;
                 }
-                umma_commit(smem_u32(&kv_empty[stage]));
-                umma_commit(smem_u32(&o_full[i & 1]));
+                if (elect_one()) mbar_arrive_one(smem_u32(&kv_empty[n % kStages]));
+                __syncwarp();
             }
-            __syncwarp();
+        } else if (mine > 0) {
+            if (!wait(q_full[PAIRED ? team : 0], 0) || (!PAIRED && !wait(q_full[1], 0))) error = 62;
+            if (!error && !scores(0)) error = 63;
+            for (int n = 0; n < mine && !error; ++n) {
+                if (n + 1 < mine && !scores(n + 1)) {
+                    error = 63;
+                    break;
+                }
+                const int stage = (kStride * n + first_block) % kStages;
+                if (!wait(p_full[team][n & 1], (n >> 1) & 1)) {
+                    error = 64;
+                    break;
+                }
+                tcgen05_fence_after();
+                const unsigned long long desc_v = smem_descriptor(v_addr + stage * L::kKvBytes);
+                if (elect_one()) {
+#pragma unroll
+                    for (int kk = 0; kk < kTtN / kUmmaK; ++kk) {
+#pragma unroll
+                        for (int half = 0; half < L::kHalves; ++half)
+                            umma_bf16_a_tmem(team_base + L::kOColumn + half * 64, team_base + L::p_column(n) + (unsigned)(kk * 8),
+                                             desc_v + (unsigned long long)(half * (L::kKvHalf >> 4) + kk * 128), idesc_o, (n > 0 || kk > 0) ? 1u : 0u);
+                    }
+                    umma_commit(smem_u32(&kv_empty[stage]));
+                    umma_commit(smem_u32(&o_full[team][n & 1]));
+                }
+                __syncwarp();
+            }
         }
     } else {
         // ------------------------------------------------------------------------------------- softmax
-        // the row's query into shared memory as TMA would lay it: 128-byte rows, 16-byte pieces exchanged by the row's low bits
-        {
-            const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(p.q) + (size_t)node * p.q_row_stride + (size_t)head * D;
+        // the rows' queries into shared memory in the products' layout: 128-byte rows, 16-byte pieces exchanged by the row's low bits
 #pragma unroll
-            for (int c = 0; c < D / 8; ++c) {
-                const uint4 v = live ? __ldg(reinterpret_cast<const uint4*>(q) + c) : make_uint4(0u, 0u, 0u, 0u);
-                const unsigned to = q_addr + (unsigned)(c >> 3) * L::kQHalf + (unsigned)row * 128u + (unsigned)(((c & 7) ^ (row & 7)) << 4);
-                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(to), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-            }
-            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-            mbar_arrive_one(smem_u32(&q_full));
+        for (int c0 = 0; c0 < kQueryPieces; ++c0) {
+            const int c = PAIRED ? c0 : team * kQueryPieces + c0;
+            const unsigned to = q_addr + (unsigned)(c >> 3) * L::kQHalf + (unsigned)lane_row * 128u + (unsigned)(((c & 7) ^ (lane_row & 7)) << 4);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(to), "r"(query[c0].x), "r"(query[c0].y), "r"(query[c0].z), "r"(query[c0].w)
+                         : "memory");
         }
-        const unsigned lane_base = tmem_base + ((unsigned)((warp & 3) * 32) << 16);
-        const unsigned* mask = p.ancestors + (size_t)node * p.words;
-        const bool warp_live = (warp & 3) * 32 < rows;
-        const float scale_log2 = p.scale * 1.4426950408889634f;
-        const float to_log2 = p.cap_out > 0.0f ? 1.4426950408889634f : scale_log2;      // (capped scores come scaled)
+        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+        mbar_arrive_one(smem_u32(&q_full[team]));
+        const bool warp_live = (row & ~31) < rows;
+        const float to_log2 = p.cap_out > 0.0f ? 1.4426950408889634f : p.scale * 1.4426950408889634f;      // (capped scores come scaled)
         const unsigned long long scale2 = pack_f32x2(to_log2, to_log2);
+        const unsigned o_taddr = row_base + L::kOColumn;
+        bool ok = true;
         // `used_max` (raw scores times to_log2) is the maximum that P and the sum are relative to; it follows the true one only
         // when that has grown by more than kSlack, so that O in tensor memory is rescaled rarely.
         constexpr float kSlack = 8.0f;
-        float used_max = -INFINITY, run_sum = 0.0f;
-        bool ok = true;
-        const unsigned o_taddr = lane_base + L::kOColumn;
-        for (int i = 0; i < blocks; ++i) {
-            ok = ok && mbar_wait(smem_u32(&s_full[i & 1]), (i >> 1) & 1);
-            ok = __all_sync(0xffffffffu, ok);
+        for (int n = 0; n < mine && !idle; ++n) {
+            const int i = kStride * n + first_block, stage = i % kStages;
+            ok = wait(s_full[team][n & 1], (n >> 1) & 1);
             if (!ok) break;
             tcgen05_fence_after();
             const int key_base = (block_begin + i) * kTtN;
-            unsigned p_packed[kTtN / 2];
+            const bool partial = key_base + kTtN > s.context || key_base < edge;
+            unsigned packed[16];
             if (!warp_live) {
 #pragma unroll
-                for (int j = 0; j < kTtN / 2; ++j) p_packed[j] = 0u;
+                for (int j = 0; j < 16; ++j) packed[j] = 0u;
+                tmem_store_16(row_base + L::p_column(n), packed);
+                tmem_store_16(row_base + L::p_column(n) + 16u, packed);
             } else {
                 float sc[kTtN];
                 {
                     unsigned lo[32], hi[32];
-                    tmem_load_32_issue(lane_base + (unsigned)((i & 1) * kTtN), lo);
-                    tmem_load_32_issue(lane_base + (unsigned)((i & 1) * kTtN + 32), hi);
+                    tmem_load_32_issue(row_base + (unsigned)((n & 1) * kTtN), lo);
+                    tmem_load_32_issue(row_base + (unsigned)((n & 1) * kTtN + 32), hi);
                     tmem_load_wait();
 #pragma unroll
                     for (int j = 0; j < 32; ++j) {
@@ -302,7 +463,7 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
 #pragma unroll
                     for (int j = 0; j < kTtN; ++j) sc[j] = p.cap_out * quick_tanh(sc[j] * p.cap_in);
                 }
-                if (key_base + kTtN > s.context || key_base < edge) {
+                if (partial) {
                     const unsigned long long seen = tree_visible(p, s, mask, position, key_base);
                     const unsigned lo = (unsigned)seen, hi = (unsigned)(seen >> 32);
 #pragma unroll
@@ -311,212 +472,284 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
                         sc[32 + j] = (hi >> j) & 1u ? sc[32 + j] : -INFINITY;
                     }
                 }
-                float part_max[4];
+                // The weights are taken relative to the maximum of the blocks before, while this block's is found: waiting for it first
+                // cost 350 cycles a step. Where it turns out larger by more than kSlack, which is rare behind a row's first blocks, O
+                // and the sum are rescaled and the weights taken once more.
+                bool settled = __any_sync(0xffffffffu, used_max == -INFINITY);
+                float largest = -INFINITY, sum;
+                if (settled) {
 #pragma unroll
-                for (int c4 = 0; c4 < 4; ++c4) {
-                    float m = max3_f32(sc[16 * c4], sc[16 * c4 + 1], sc[16 * c4 + 2]);
-#pragma unroll
-                    for (int j = 3; j < 15; j += 2) m = max3_f32(m, sc[16 * c4 + j], sc[16 * c4 + j + 1]);
-                    part_max[c4] = fmaxf(m, sc[16 * c4 + 15]);
+                    for (int j = 0; j < kTtN; j += 2) largest = max3_f32(largest, sc[j], sc[j + 1]);
                 }
-                // (a negative scale turns the order round: the largest is then found among the scaled ones)
-                float block_max = fmaxf(max3_f32(part_max[0], part_max[1], part_max[2]), part_max[3]) * to_log2;
-                if (to_log2 <= 0.0f) {
-                    block_max = -INFINITY;
+                bool raise = settled;
+                while (true) {
+                    if (raise) {
+                        const float new_max = fmaxf(used_max, largest * to_log2);
+                        const bool grown = new_max > used_max + kSlack;      // (-inf + slack = -inf)
+                        if (n > 0 && __any_sync(0xffffffffu, grown)) {
+                            ok = wait(o_full[team][(n - 1) & 1], ((n - 1) >> 1) & 1);
+                            if (!ok) break;
+                            tcgen05_fence_after();
+                            const float factor = !grown ? 1.0f : (used_max == -INFINITY ? 0.0f : exp2f(used_max - new_max));
+                            const unsigned long long factor2 = pack_f32x2(factor, factor);
 #pragma unroll
-                    for (int j = 0; j < kTtN; ++j) block_max = sc[j] == -INFINITY ? block_max : fmaxf(block_max, sc[j] * to_log2);
-                }
-                if (i == 0) {
-                    used_max = block_max;
-                } else {
-                    const float new_max = fmaxf(used_max, block_max);
-                    const bool grown = new_max > used_max + kSlack;          // (-inf + slack = -inf)
-                    if (__any_sync(0xffffffffu, grown)) {
-                        ok = mbar_wait(smem_u32(&o_full[(i - 1) & 1]), ((i - 1) >> 1) & 1);
-                        ok = __all_sync(0xffffffffu, ok);
-                        if (!ok) break;
-                        tcgen05_fence_after();
-                        const float factor = !grown ? 1.0f : (used_max == -INFINITY ? 0.0f : exp2f(used_max - new_max));
-                        const unsigned long long factor2 = pack_f32x2(factor, factor);
+                            for (int c0 = 0; c0 < D; c0 += 16) {
+                                unsigned part[16];
+                                tmem_load_16_issue(o_taddr + (unsigned)c0, part);
+                                tmem_load_wait();
 #pragma unroll
-                        for (int c0 = 0; c0 < D; c0 += 32) {
-                            unsigned part[32];
-                            tmem_load_32_issue(o_taddr + (unsigned)c0, part);
-                            tmem_load_wait();
-#pragma unroll
-                            for (int j = 0; j < 32; j += 2) {
-                                float a, b;
-                                unpack_f32x2(mul_f32x2(pack_f32x2(__uint_as_float(part[j]), __uint_as_float(part[j + 1])), factor2), a, b);
-                                part[j] = __float_as_uint(a);
-                                part[j + 1] = __float_as_uint(b);
+                                for (int j = 0; j < 16; j += 2) {
+                                    float a, b;
+                                    unpack_f32x2(mul_f32x2(pack_f32x2(__uint_as_float(part[j]), __uint_as_float(part[j + 1])), factor2), a, b);
+                                    part[j] = __float_as_uint(a);
+                                    part[j + 1] = __float_as_uint(b);
+                                }
+                                tmem_store_16(o_taddr + (unsigned)c0, part);
                             }
-                            tmem_store_32(o_taddr + (unsigned)c0, part);
+                            run_sum *= factor;
                         }
-                        tmem_store_wait();
-                        run_sum *= factor;
-                        if (grown) used_max = new_max;
+                        if (grown || used_max == -INFINITY) used_max = new_max;
                     }
+                    const float base = used_max == -INFINITY ? 0.0f : used_max;
+                    const unsigned long long neg_base2 = pack_f32x2(-base, -base);
+                    largest = -INFINITY;
+                    sum = tree_weights(sc, scale2, neg_base2, packed, largest);
+                    tmem_store_16(row_base + L::p_column(n), packed);
+                    sum += tree_weights(sc + 32, scale2, neg_base2, packed, largest);
+                    tmem_store_16(row_base + L::p_column(n) + 16u, packed);
+                    if (settled) break;
+                    settled = true;
+                    raise = __any_sync(0xffffffffu, largest * to_log2 > used_max + kSlack);
+                    if (!raise) break;
                 }
-                const float safe_max = used_max == -INFINITY ? 0.0f : used_max;
-                const unsigned long long neg_max2 = pack_f32x2(-safe_max, -safe_max);
-                unsigned long long part_sum[4] = {0ull, 0ull, 0ull, 0ull};          // (0.0f, 0.0f) each
-                const bool turned = to_log2 <= 0.0f;
-#pragma unroll
-                for (int j2 = 0; j2 < kTtN / 2; ++j2) {
-                    float x0, x1, a, b;
-                    unpack_f32x2(fma_f32x2(pack_f32x2(sc[2 * j2], sc[2 * j2 + 1]), scale2, neg_max2), x0, x1);
-                    if (turned) {
-                        x0 = sc[2 * j2] == -INFINITY ? -INFINITY : x0;
-                        x1 = sc[2 * j2 + 1] == -INFINITY ? -INFINITY : x1;
-                    }
-                    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(x0));
-                    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(b) : "f"(x1));
-                    const __nv_bfloat162 pair = __floats2bfloat162_rn(a, b);          // key 2 j2 in the lower half
-                    const unsigned packed = *reinterpret_cast<const unsigned*>(&pair);
-                    p_packed[j2] = packed;
-                    part_sum[j2 & 3] = add_f32x2(part_sum[j2 & 3], pack_f32x2(__uint_as_float(packed << 16), __uint_as_float(packed & 0xffff0000u)));
-                }
-                float s0, s1;
-                unpack_f32x2(add_f32x2(add_f32x2(part_sum[0], part_sum[1]), add_f32x2(part_sum[2], part_sum[3])), s0, s1);
-                run_sum += s0 + s1;
-            }
-            // (K and V of a block came together: its scores being there, its values are)
-            if (key_base + kTtN > s.context || key_base < edge) {
-                const int stage = i % kStages;
-                ok = mbar_wait(smem_u32(&kv_full[stage]), (i / kStages) & 1);
-                ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
-                // values of places that hold no key of this span become zeros, as do those that are not finite: two threads a row
-                const int key = key_base + row / 2;
-                const bool none = key < first_key || key > last_key;
+                run_sum += sum;
+            }
+            tmem_store_wait();
+            if (partial) {
+                // values that are not finite are taken out: two threads a row
+                ok = wait(kv_full[stage], (i / kStages) & 1);
+                if (!ok) break;
                 bool found = false;
 #pragma unroll
                 for (int half = 0; half < L::kHalves; ++half)
 #pragma unroll
                     for (int c = 0; c < 64; c += 16) {
-                        const unsigned at = v_addr + stage * L::kKvBytes + half * L::kKvHalf + (unsigned)(row * 64 + c);
+                        const unsigned at = v_addr + stage * L::kKvBytes + half * L::kKvHalf + (unsigned)(lane_row * 64 + c);
                         unsigned w[4];
                         asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
-                        bool change = none;
+                        bool change = false;
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const bool low = none || not_finite(w[e] & 0xffffu), high = none || not_finite(w[e] >> 16);
+                            const bool low = not_finite(w[e] & 0xffffu), high = not_finite(w[e] >> 16);
                             change |= low | high;
                             w[e] = (low ? 0u : w[e] & 0xffffu) | (high ? 0u : w[e] & 0xffff0000u);
                         }
                         if (change) asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
-                        found |= change && !none;
+                        found |= change;
                     }
                 if (found) bad_values = 1;
                 asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
             }
-            tmem_store_32(lane_base + L::p_column(i), p_packed);
-            tmem_store_wait();
             tcgen05_fence_before();
-            mbar_arrive_one(smem_u32(&p_full[i & 1]));
+            mbar_arrive_one(smem_u32(&p_full[team][n & 1]));
         }
-        if (ok && blocks > 0) {
-            ok = mbar_wait(smem_u32(&o_full[(blocks - 1) & 1]), ((blocks - 1) >> 1) & 1);
-            ok = __all_sync(0xffffffffu, ok);
-            if (ok) tcgen05_fence_after();
-        }
-        if (!ok) {
-            if (lane == 0) atomicExch(p.error_flag, 65);
-        } else {
-            const size_t unit = (size_t)node * p.q_heads + head;
-            float inv = 1.0f;
-            if (p.splits > 1) {
-                if (live) {
-                    p.part_ml[(unit * p.splits + split) * 2] = used_max;
-                    p.part_ml[(unit * p.splits + split) * 2 + 1] = run_sum;
-                }
-            } else {
-                const float sink_part = (p.sinks && used_max != -INFINITY) ? exp2f(p.sinks[head] * 1.4426950408889634f - used_max) : 0.0f;
-                inv = used_max == -INFINITY ? 0.0f : 1.0f / (run_sum + sink_part);
-            }
-            // every softmax thread has passed its last look at the values (o_full came after all of their arrivals)
-            const bool bad = *reinterpret_cast<volatile int*>(&bad_values) != 0;
-#pragma unroll
+        if (ok && mine > 0 && !idle) ok = wait(o_full[team][(mine - 1) & 1], ((mine - 1) >> 1) & 1);
+        if (!ok) error = 65;
+    }
+    if (error) atomicExch(p.error_flag, error);
+
+    // ---- what the teams have, of all pieces of the keys, meets in shared memory, where queries and keys were: every block of the
+    // cluster owns some of the rows, and everybody writes a row's part (outputs, maximum, sum) to its owner
+    const bool across = p.splits > 1 && p.part_o == nullptr;    // the pieces of the keys are a cluster
+    const int pieces = across ? p.splits : 1, parts = PAIRED ? pieces : 2 * pieces;
+    const int row_first = across ? split * rows / p.splits : 0, count = (across ? (split + 1) * rows / p.splits : rows) - row_first;
+    const int most = (rows + pieces - 1) / pieces;              // rows of an owner
+    tcgen05_fence_before();
+    __syncthreads();                                            // (every product of the block is done, every copy has landed)
+    if (across) cluster_sync();
+    tcgen05_fence_after();
+    const unsigned stats_at = smem_base + L::kStatsAt;          // [part][most] pairs; outputs before: [part][most][kPitch]
+    if (softmax && !idle) {
+        const int owner = across ? ((row + 1) * p.splits - 1) / rows : 0;
+        const int slot = (PAIRED ? (across ? split : 0) : (across ? 2 * split : 0) + team) * most + row - (across ? owner * rows / p.splits : 0);
+        const unsigned stats_to = peer_address(stats_at + (unsigned)slot * 8u, owner, across && live);
+        const unsigned to = peer_address(smem_base + (unsigned)(slot * L::kPitch) * 4u, owner, across && live);
+        if (live) store_2(stats_to, used_max, run_sum);
+        const bool bad = bad_values != 0;
+        if (mine > 0) {
+#pragma unroll 1
             for (int c0 = 0; c0 < D; c0 += 32) {
                 unsigned o[32];
-                __syncwarp();
-                if (blocks > 0) {
-                    tmem_load_32_issue(o_taddr + (unsigned)c0, o);
-                    tmem_load_wait();
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) o[j] = 0u;
-                }
+                __syncwarp();                                   // (a load from tensor memory wants the whole warp)
+                tmem_load_32_issue(row_base + L::kOColumn + (unsigned)c0, o);
+                tmem_load_wait();
                 if (!live) continue;
                 if (bad) {
-                    for (int i = 0; i < blocks; ++i) {
+                    const int* table = p.block_table + (size_t)span * p.table_stride;
+                    for (int i = first_block; i < blocks; i += kStride) {
                         const int key_base = (block_begin + i) * kTtN;
                         if (key_base + kTtN <= s.context && key_base >= edge) continue;
-                        const int* table = p.block_table + (size_t)span * p.table_stride;
                         for (unsigned long long seen = tree_visible(p, s, mask, position, key_base); seen; seen &= seen - 1) {
                             const int key = key_base + __ffsll((long long)seen) - 1;
                             const int logical = key / p.page_tokens;
                             const int page = logical < p.table_stride ? table[logical] : -1;
                             if (page < 0 || page >= p.pages) continue;
                             const __nv_bfloat16* v = static_cast<const __nv_bfloat16*>(p.v_cache) + (long long)page * p.page_stride +
-                                                     ((long long)kvh * p.page_tokens + key % p.page_tokens) * D + c0;
+                                                     ((long long)kvh * p.page_tokens + key % p.page_tokens) * d + c0;
 #pragma unroll
                             for (int j = 0; j < 32; ++j) {
-                                const float x = __bfloat162float(v[j]);
+                                const float x = c0 + j < d ? __bfloat162float(v[j]) : 0.0f;
                                 if (!isfinite(x)) o[j] = __float_as_uint(__uint_as_float(o[j]) + x);
                             }
                         }
                     }
                 }
-                if (p.splits > 1) {
-                    float* dst = p.part_o + (unit * p.splits + split) * D + c0;
-                    if (used_max != -INFINITY) {
 #pragma unroll
-                        for (int c = 0; c < 32; c += 4) *reinterpret_cast<uint4*>(dst + c) = make_uint4(o[c], o[c + 1], o[c + 2], o[c + 3]);
-                    }
-                } else {
-                    __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.out) + unit * D + c0;
-#pragma unroll
-                    for (int c = 0; c < 32; c += 8) {
-                        uint4 packed;
-                        __nv_bfloat162* h2 = reinterpret_cast<__nv_bfloat162*>(&packed);
-#pragma unroll
-                        for (int e2 = 0; e2 < 4; ++e2)
-                            h2[e2] = __floats2bfloat162_rn(__uint_as_float(o[c + 2 * e2]) * inv, __uint_as_float(o[c + 2 * e2 + 1]) * inv);
-                        *reinterpret_cast<uint4*>(dst + c) = packed;
-                    }
-                }
+                for (int c = 0; c < 32; c += 4) store_4(to + (unsigned)(c0 + c) * 4u, o[c], o[c + 1], o[c + 2], o[c + 3]);
             }
             __syncwarp();
         }
     }
-    if (error) atomicExch(p.error_flag, error);
     tcgen05_fence_before();
+    if (across)
+        cluster_sync();
+    else
+        __syncthreads();
+    if (warp == kTtCopyWarps) tmem_dealloc(tmem_base, kTtTmemColumns);
+    // The owner's rows: first the parts' maxima and sums become their factors, a thread a row, then the outputs are added up, eight
+    // columns at a time, the parts in order. (Loops short in instructions: this runs once a block, and fetching what it takes for
+    // the first time costs more than running it.)
+    unsigned char* meeting = smem_raw + (smem_base - smem_u32(smem_raw));
+    const float* meet = reinterpret_cast<const float*>(meeting);
+    float2* row_stats = reinterpret_cast<float2*>(meeting + L::kStatsAt);
+    int* unit_s = reinterpret_cast<int*>(meeting + L::kUnitsAt);
+    if (tid < count) {
+        float top = -INFINITY, sum = 0.0f;
+#pragma unroll 1
+        for (int part = 0; part < parts; ++part) top = fmaxf(top, row_stats[part * most + tid].x);
+#pragma unroll 1
+        for (int part = 0; part < parts; ++part) {
+            const float2 stats = row_stats[part * most + tid];
+            const float factor = stats.x == -INFINITY ? 0.0f : fast_exp2(stats.x - top);
+            sum = fmaf(stats.y, factor, sum);
+            row_stats[part * most + tid].x = factor;
+        }
+        const int of_row = row0 + row_first + tid, of_head = kvh * p.group + of_row % p.group;
+        const int unit = (s.begin + of_row / p.group) * p.q_heads + of_head;      // (fits: see tree_tcgen05_takes)
+        unit_s[tid] = unit;
+        float inv = 1.0f;
+        if (p.part_o) {
+            *reinterpret_cast<float2*>(p.part_ml + ((size_t)unit * p.splits + split) * 2) = make_float2(top, sum);
+        } else {
+            if (p.sinks && top != -INFINITY) sum += fast_exp2(p.sinks[of_head] * 1.4426950408889634f - top);
+            inv = top == -INFINITY ? 0.0f : 1.0f / sum;
+        }
+#pragma unroll 1
+        for (int part = 0; part < parts; ++part) row_stats[part * most + tid].y = inv;
+    }
     __syncthreads();
-    if (warp == 0) tmem_dealloc(tmem_base, kTtTmemColumns);
+#pragma unroll 1
+    for (int item = tid; item < count * (D / 8); item += kTtThreads) {
+        const int r = item / (D / 8), c = item % (D / 8) * 8;
+        if (c >= d) continue;
+        float4 lo = make_float4(0.0f, 0.0f, 0.0f, 0.0f), hi = lo;
+#pragma unroll 2
+        for (int part = 0; part < parts; ++part) {
+            const float factor = row_stats[part * most + r].x;
+            if (factor == 0.0f) continue;                       // (a part without keys of the row has left nothing)
+            const float4* at = reinterpret_cast<const float4*>(meet + (part * most + r) * L::kPitch + c);
+            const float4 x = at[0], y = at[1];
+            lo = make_float4(fmaf(x.x, factor, lo.x), fmaf(x.y, factor, lo.y), fmaf(x.z, factor, lo.z), fmaf(x.w, factor, lo.w));
+            hi = make_float4(fmaf(y.x, factor, hi.x), fmaf(y.y, factor, hi.y), fmaf(y.z, factor, hi.z), fmaf(y.w, factor, hi.w));
+        }
+        const float inv = row_stats[r].y;
+        const size_t unit = unit_s[r];
+        if (p.part_o) {
+            float4* to = reinterpret_cast<float4*>(p.part_o + (unit * p.splits + split) * d + c);
+            to[0] = lo;
+            to[1] = hi;
+        } else {
+            *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + unit * d + c) =
+                make_uint4(pack_bf16_pair(lo.x * inv, lo.y * inv), pack_bf16_pair(lo.z * inv, lo.w * inv),
+                           pack_bf16_pair(hi.x * inv, hi.y * inv), pack_bf16_pair(hi.z * inv, hi.w * inv));
+        }
+    }
 }
 
 bool tree_tcgen05_takes(const TreeParams& p) {
-    return (p.head_dim == 64 || p.head_dim == 128) && p.page_tokens >= 8 && p.page_tokens % 8 == 0 && kTtN % p.page_tokens == 0 &&
-           p.page_stride == (long long)p.kv_heads * p.page_tokens * p.head_dim && p.q_row_stride % 8 == 0 &&
-           (((size_t)p.q | (size_t)p.k_cache | (size_t)p.v_cache | (size_t)p.out) & 15) == 0 && ((size_t)p.part_o & 15) == 0 &&
-           (long long)p.pages * p.kv_heads * p.page_tokens < (1ll << 31);
+    // (page strides and (token, query head) numbers of 32 bits)
+    return p.head_dim % 8 == 0 && p.page_stride < (1ll << 32) && (long long)p.tokens * p.q_heads < (1ll << 31) && p.head_dim <= 128 && p.page_stride % 8 == 0 && p.q_row_stride % 8 == 0 && p.scale > 0.0f &&
+           (((size_t)p.q | (size_t)p.k_cache | (size_t)p.v_cache | (size_t)p.out | (size_t)p.part_o) & 15) == 0;
 }
 
-int tree_tcgen05_rows() { return kTtM; }
+// Two teams' rows a tile where one tile of 128 does not hold them: the same keys would be read for every tile.
+static bool tree_paired(const TreeParams& p) { return p.max_nodes * p.group > kTtM; }
+
+template <int D, bool PAIRED>
+static cudaError_t tree_config(cudaLaunchConfig_t& config, cudaLaunchAttribute (&attributes)[2], int cluster) {
+    constexpr unsigned smem = TtLayout<D, PAIRED>::kSmemBytes;
+    const cudaError_t status = cudaFuncSetAttribute(attention_tree_tcgen05_kernel<D, PAIRED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    config.blockDim = dim3(kTtThreads);
+    config.dynamicSmemBytes = smem;
+    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[0].val.programmaticStreamSerializationAllowed = chaining_enabled() ? 1 : 0;
+    attributes[1].id = cudaLaunchAttributeClusterDimension;
+    attributes[1].val.clusterDim = {(unsigned)cluster, 1, 1};
+    config.attrs = attributes;
+    config.numAttrs = cluster > 1 ? 2 : 1;
+    return status;
+}
+
+// How many clusters of `size` blocks the device runs at a time (a cluster wants SMs of one group: 148 SMs hold fewer than
+// 148 / size). Asked once; any device of this kind answers alike.
+template <int D, bool PAIRED>
+static int clusters_at_once(int size) {
+    static std::atomic<int> known[kTtMaxCluster + 1];
+    int count = known[size].load(std::memory_order_relaxed);
+    if (count == 0) {
+        cudaLaunchConfig_t config = {};
+        cudaLaunchAttribute attributes[2];
+        config.gridDim = dim3(size, 1, 1);
+        if (tree_config<D, PAIRED>(config, attributes, size) != cudaSuccess ||
+            cudaOccupancyMaxActiveClusters(&count, attention_tree_tcgen05_kernel<D, PAIRED>, &config) != cudaSuccess || count <= 0) {
+            cudaGetLastError();
+            count = 148 / size;
+        }
+        known[size].store(count, std::memory_order_relaxed);
+    }
+    return count;
+}
+
+template <int D, bool PAIRED>
+static TreeTile tree_tile() {
+    TreeTile tile = {PAIRED ? 2 * kTtM : kTtM, 148, 14, kTtMaxCluster, {0}};
+    for (int size = 2; size <= kTtMaxCluster; ++size) tile.problems_at_once[size] = clusters_at_once<D, PAIRED>(size);
+    return tile;
+}
+
+TreeTile tree_tcgen05_tile(const TreeParams& p) {
+    if (p.head_dim <= 64) return tree_paired(p) ? tree_tile<64, true>() : tree_tile<64, false>();
+    return tree_paired(p) ? tree_tile<128, true>() : tree_tile<128, false>();
+}
+
+template <int D, bool PAIRED>
+static int launch_tree(const TreeParams& p, cudaStream_t stream) {
+    cudaLaunchConfig_t config = {};
+    cudaLaunchAttribute attributes[2];
+    cudaError_t status = tree_config<D, PAIRED>(config, attributes, p.part_o ? 1 : p.splits);
+    CELEG_REQUIRE(status == cudaSuccess, "attention_tree: %s", cudaGetErrorString(status));
+    const int tile = PAIRED ? 2 * kTtM : kTtM, tiles = (p.max_nodes * p.group + tile - 1) / tile;
+    config.gridDim = dim3(tiles * p.splits, p.kv_heads, p.spans);
+    config.stream = stream;
+    status = cudaLaunchKernelEx(&config, attention_tree_tcgen05_kernel<D, PAIRED>, p);
+    CELEG_REQUIRE(status == cudaSuccess, "attention_tree: %s", cudaGetErrorString(status));
+    return check_launch("attention_tree");
+}
 
 int launch_tree_tcgen05(const TreeParams& p, cudaStream_t stream) {
-    CUtensorMap map_k, map_v;
-    const long long cache_rows = (long long)p.pages * p.kv_heads * p.page_tokens;
-    if (!tensor_map_for(p.k_cache, cache_rows, p.head_dim, p.head_dim, p.page_tokens, &map_k)) return -2;
-    if (!tensor_map_for(p.v_cache, cache_rows, p.head_dim, p.head_dim, p.page_tokens, &map_v)) return -2;
-    auto kernel = p.head_dim == 64 ? attention_tree_tcgen05_kernel<64> : attention_tree_tcgen05_kernel<128>;
-    const unsigned smem = p.head_dim == 64 ? TtLayout<64>::kSmemBytes : TtLayout<128>::kSmemBytes;
-    const cudaError_t status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    CELEG_REQUIRE(status == cudaSuccess, "attention_tree: %s", cudaGetErrorString(status));
-    const int tiles = (p.max_nodes * p.group + kTtM - 1) / kTtM;
-    kernel<<<dim3(tiles * p.splits, p.kv_heads, p.spans), kTtThreads, smem, stream>>>(map_k, map_v, p);
-    return check_launch("attention_tree");
+    if (p.head_dim <= 64) return tree_paired(p) ? launch_tree<64, true>(p, stream) : launch_tree<64, false>(p, stream);
+    return tree_paired(p) ? launch_tree<128, true>(p, stream) : launch_tree<128, false>(p, stream);
 }
 
 }  // namespace celeg_b200
