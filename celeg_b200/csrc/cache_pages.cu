@@ -5,6 +5,8 @@
 // Caches: [layers, pages, kv_heads, page_tokens, row], a row being the bytes of one head at one position.
 #include "common.cuh"
 
+#include <cstdlib>
+
 namespace celeg_b200 {
 
 struct CacheSide {
@@ -72,6 +74,34 @@ static int piece_bytes(const CacheSide& k, const CacheSide& v) {
     for (int bytes = 16; bytes > 2; bytes /= 2)
         if ((bits & (bytes - 1)) == 0) return bytes;
     return 2;
+}
+
+// The first move that writes a page which another move writes, or reads one which another move writes; -1: none, -2: no memory.
+// A table of the written pages, open addressing, at most half full; the usual lists' on the stack.
+static int clashing_move(const PageMove* list, int count) {
+    constexpr int kOnStack = 4096;
+    int on_stack[kOnStack];
+    long long size = 16;
+    while (size < 2ll * count) size *= 2;
+    int* table = size <= kOnStack ? on_stack : static_cast<int*>(malloc((size_t)size * sizeof(int)));
+    if (!table) return -2;
+    const unsigned mask = (unsigned)(size - 1);
+    for (long long i = 0; i < size; ++i) table[i] = -1;
+    int clash = -1;
+    auto place = [&](int page) {
+        unsigned at = ((unsigned)page * 2654435761u) >> 7 & mask;
+        while (table[at] >= 0 && table[at] != page) at = (at + 1) & mask;
+        return at;
+    };
+    for (int i = 0; i < count && clash < 0; ++i) {
+        const unsigned at = place(list[i].to);
+        if (table[at] >= 0) clash = i;
+        table[at] = list[i].to;
+    }
+    for (int i = 0; i < count && clash < 0; ++i)
+        if (list[i].from != list[i].to && table[place(list[i].from)] >= 0) clash = i;
+    if (table != on_stack) free(table);
+    return clash;
 }
 
 // ------------------------------------------------------------------------------------------------ accepted drafts
@@ -231,6 +261,10 @@ CELEG_API int celeg_copy_pages(void* k, long long k_layer_stride, long long k_pa
                       "copy_pages: move %d (page %d to %d, %d positions) is outside %d pages of %d", i, list[i].from, list[i].to,
                       list[i].rows, pages, page_tokens);
     if (count == 0 || (!ks.base && !vs.base)) return 0;
+    const int clash = clashing_move(list, count);
+    CELEG_REQUIRE(clash != -2, "copy_pages: no memory to check %d moves", count);
+    CELEG_REQUIRE(clash < 0, "copy_pages: move %d (page %d to %d) writes a page that another one writes, or reads one that another one writes",
+                  clash, list[clash < 0 ? 0 : clash].from, list[clash < 0 ? 0 : clash].to);
     const int piece = piece_bytes(ks, vs);
     for (int done = 0; done < count;) {
         const int now = count - done > kManyMoves ? kManyMoves : count - done;

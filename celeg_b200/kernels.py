@@ -857,24 +857,25 @@ def _refuse(what: str) -> None:
     raise KernelLibraryError(what)
 
 
-def _here(operator: str, *tensors: Optional[torch.Tensor]) -> None:
-    """Every tensor on the current CUDA device, whose current stream the launch goes to."""
-    device = None
-    for tensor in tensors:
-        if tensor is None:
-            continue
-        if not tensor.is_cuda:
-            _refuse(f"{operator}: a tensor on {tensor.device}, CUDA tensors are needed")
-        if device is None:
-            device = torch._C._cuda_getDevice()
+_I32 = torch.int32
+
+
+def _check_vectors(operator: str, device: int, vectors) -> None:
+    """``vectors``: (name, tensor, least number of elements, type) of contiguous tensors on CUDA device ``device``, which has to
+    be the current one: the launch goes to its current stream."""
+    for name, tensor, elements, dtype in vectors:
+        if tensor.dtype is not dtype or tensor.numel() < elements or not tensor.is_contiguous():
+            _refuse(f"{operator}: {name} must be a contiguous tensor of {dtype} with at least {elements} elements, got "
+                    f"{tuple(tensor.shape)} of {tensor.dtype}, contiguous={tensor.is_contiguous()}")
         if tensor.get_device() != device:
-            _refuse(f"{operator}: a tensor on {tensor.device} while the current device is cuda:{device}")
+            _refuse(f"{operator}: {name} on {tensor.device}, other tensors on device {device}")
+    if device < 0 or device != torch._C._cuda_getDevice():
+        _refuse(f"{operator}: tensors of CUDA device {device}, which must be the current one")
 
 
-def _vector32(operator: str, tensor: torch.Tensor, elements: int, name: str, dtype: torch.dtype = torch.int32) -> None:
-    if tensor.dtype != dtype or not tensor.is_contiguous() or tensor.numel() < elements:
-        _refuse(f"{operator}: {name} must be a contiguous tensor of {dtype} with at least {elements} elements, got "
-                f"{tuple(tensor.shape)} of {tensor.dtype}, contiguous={tensor.is_contiguous()}")
+def _check_table(operator: str, table: torch.Tensor, spans: int) -> None:
+    if table.dim() != 2 or table.shape[0] < spans or table.dtype is not _I32 or table.stride(1) != 1:
+        _refuse(f"{operator}: a block table {tuple(table.shape)} of {table.dtype} for {spans} spans")
 
 
 def attention_tree_scratch(device) -> torch.Tensor:
@@ -902,33 +903,33 @@ def attention_tree(q: torch.Tensor, q_row_stride: int, out: torch.Tensor, k_cach
     name = "attention_tree"
     dtype = q.dtype
     code = dtype_code(dtype)
-    if k_cache.dtype != dtype or v_cache.dtype != dtype or out.dtype != dtype:
-        _refuse(f"{name}: q {dtype}, caches {k_cache.dtype} and {v_cache.dtype}, out {out.dtype}")
-    page = (kv_heads, page_tokens, head_dim)
-    inner = (page_tokens * head_dim, head_dim, 1)
-    if (k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[1:] != page or k_cache.stride()[1:] != inner
-            or v_cache.stride() != k_cache.stride()):
-        _refuse(f"{name}: caches [pages, kv_heads, page_tokens, head_dim] of pages {page} are needed, got {tuple(k_cache.shape)} and "
-                f"{tuple(v_cache.shape)} with strides {k_cache.stride()} and {v_cache.stride()}")
-    if q.dim() != 2 or q.stride(1) != 1 or q.shape[0] < tokens or q.shape[1] < q_heads * head_dim or (tokens > 1 and q.stride(0) != q_row_stride):
+    if k_cache.dtype is not dtype or v_cache.dtype is not dtype:
+        _refuse(f"{name}: q {dtype}, caches {k_cache.dtype} and {v_cache.dtype}")
+    strides = k_cache.stride()
+    shape = k_cache.shape
+    if (shape[1:] != (kv_heads, page_tokens, head_dim) or strides[1:] != (page_tokens * head_dim, head_dim, 1) or v_cache.shape != shape
+            or v_cache.stride() != strides):
+        _refuse(f"{name}: caches [pages, kv_heads, page_tokens, head_dim] with pages {(kv_heads, page_tokens, head_dim)} in one piece are "
+                f"needed, got {tuple(shape)} and {tuple(v_cache.shape)} with strides {strides} and {v_cache.stride()}")
+    if (q.dim() != 2 or q.stride(1) != 1 or q.shape[0] < tokens or q.shape[1] < q_heads * head_dim
+            or (tokens > 1 and q.stride(0) != q_row_stride)):
         _refuse(f"{name}: q {tuple(q.shape)} with strides {q.stride()} does not hold {tokens} rows of {q_heads} x {head_dim}, {q_row_stride} apart")
-    _vector32(name, out, tokens * q_heads * head_dim, "out", dtype)
-    _vector32(name, positions, tokens, "positions")
-    _vector32(name, span_begin, spans + 1, "span_begin")
-    _vector32(name, span_context, spans, "span_context")
-    _vector32(name, error_flag, 1, "error_flag")
     if ancestors.dim() != 2 or ancestors.shape[0] < tokens:
         _refuse(f"{name}: ancestors {tuple(ancestors.shape)} for {tokens} tokens")
-    _vector32(name, ancestors, 0, "ancestors")
-    if block_table.dim() != 2 or block_table.shape[0] < spans or block_table.dtype != torch.int32 or block_table.stride(1) != 1:
-        _refuse(f"{name}: a block table {tuple(block_table.shape)} of {block_table.dtype} for {spans} spans")
+    _check_table(name, block_table, spans)
+    device = q.get_device()
+    vectors = [("out", out, tokens * q_heads * head_dim, dtype), ("positions", positions, tokens, _I32),
+               ("span_begin", span_begin, spans + 1, _I32), ("span_context", span_context, spans, _I32),
+               ("ancestors", ancestors, 0, _I32), ("error_flag", error_flag, 1, _I32)]
     if sinks is not None:
-        _vector32(name, sinks, q_heads, "sinks", torch.float32)
+        vectors.append(("sinks", sinks, q_heads, torch.float32))
     if scratch is not None:
-        _vector32(name, scratch, 0, "scratch", torch.float32)
-    _here(name, q, out, k_cache, v_cache, positions, span_begin, span_context, ancestors, block_table, error_flag, sinks, scratch)
+        vectors.append(("scratch", scratch, 0, torch.float32))
+    if k_cache.get_device() != device or v_cache.get_device() != device or block_table.get_device() != device:
+        _refuse(f"{name}: q on {q.device}, caches on {k_cache.device} and {v_cache.device}, block table on {block_table.device}")
+    _check_vectors(name, device, vectors)
     _check(library().celeg_attention_tree(
-        q.data_ptr(), q_row_stride, out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0), k_cache.shape[0],
+        q.data_ptr(), q_row_stride, out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), strides[0], shape[0],
         positions.data_ptr(), span_begin.data_ptr(), span_context.data_ptr(), ancestors.data_ptr(), ancestors.shape[1],
         block_table.data_ptr(), block_table.stride(0), tokens, spans, max_nodes, max_keys, q_heads, kv_heads, head_dim,
         page_tokens, int(window or 0), scale, _ptr(sinks), float(softcap or 0.0), _ptr(scratch),
@@ -937,17 +938,20 @@ def attention_tree(q: torch.Tensor, q_row_stride: int, out: torch.Tensor, k_cach
 
 def _cache_sides(operator: str, k: torch.Tensor, v: torch.Tensor) -> tuple:
     """What the entry points that move cached rows are given of keys and values [layers, pages, kv_heads, page_tokens, *]."""
-    if k.dim() != 5 or v.dim() != 5 or k.shape[:4] != v.shape[:4] or k.dtype != v.dtype:
-        _refuse(f"{operator}: keys and values [layers, pages, kv_heads, page_tokens, *] of one type are needed, got {tuple(k.shape)} of "
-                f"{k.dtype} and {tuple(v.shape)} of {v.dtype}")
-    layers, pages, heads, page_tokens = k.shape[:4]
-    dtype_code(k.dtype)
-    for side in (k, v):
-        dim = side.shape[4]
-        if side.numel() and side.stride()[2:] != (page_tokens * dim, dim, 1):
-            _refuse(f"{operator}: a page's heads, positions and numbers must lie side by side, got strides {side.stride()} of {tuple(side.shape)}")
-    return (k.data_ptr(), k.stride(0), k.stride(1), k.shape[4], v.data_ptr(), v.stride(0), v.stride(1), v.shape[4], layers, pages,
-            heads, page_tokens, k.element_size())
+    k_shape, v_shape, k_strides, v_strides = k.shape, v.shape, k.stride(), v.stride()
+    if len(k_shape) != 5 or k_shape[:4] != v_shape[:4] or len(v_shape) != 5 or k.dtype is not v.dtype:
+        _refuse(f"{operator}: keys and values [layers, pages, kv_heads, page_tokens, *] of one type are needed, got {tuple(k_shape)} of "
+                f"{k.dtype} and {tuple(v_shape)} of {v.dtype}")
+    layers, pages, heads, page_tokens, k_dim = k_shape
+    v_dim = v_shape[4]
+    element = 4 if dtype_code(k.dtype) == FLOAT32 else 2
+    if (k_dim and k_strides[2:] != (page_tokens * k_dim, k_dim, 1)) or (v_dim and v_strides[2:] != (page_tokens * v_dim, v_dim, 1)):
+        _refuse(f"{operator}: a page's heads, positions and numbers must lie side by side, got strides {k_strides} of {tuple(k_shape)} "
+                f"and {v_strides} of {tuple(v_shape)}")
+    if k.get_device() != v.get_device():
+        _refuse(f"{operator}: keys on {k.device}, values on {v.device}")
+    return (k.data_ptr(), k_strides[0], k_strides[1], k_dim, v.data_ptr(), v_strides[0], v_strides[1], v_dim, layers, pages,
+            heads, page_tokens, element)
 
 
 def copy_pages(k: torch.Tensor, v: torch.Tensor, moves) -> None:
@@ -956,22 +960,18 @@ def copy_pages(k: torch.Tensor, v: torch.Tensor, moves) -> None:
     lies behind them stays. A page may be read by many moves; none may be written twice, or written by one and read by
     another. ``k``, ``v``: [layers, pages, kv_heads, page_tokens, *]."""
     sides = _cache_sides("copy_pages", k, v)
-    if len(moves) == 0:
+    table = moves if isinstance(moves, np.ndarray) else np.asarray(moves)
+    if table.size == 0:
         return
-    table = np.ascontiguousarray(moves)
     if table.ndim != 2 or table.shape[1] != 3 or table.dtype.kind not in "iu":
         _refuse(f"copy_pages: moves are triples of whole numbers (from, to, positions), got {table.dtype} {table.shape}")
-    if table.min() < 0 or table.max() >= 1 << 31:
-        _refuse("copy_pages: a page or a number of positions is negative or too large")
-    listed = table.tolist()
-    written = {to for _, to, _ in listed}
-    if len(written) != len(listed):
-        _refuse("copy_pages: a page is written by two moves")
-    if any(source in written and source != to for source, to, _ in listed):
-        _refuse("copy_pages: a page is written by one move and read by another")
-    _here("copy_pages", k, v)
-    table = np.ascontiguousarray(table, dtype=np.int32)
-    _check(library().celeg_copy_pages(*sides, table.ctypes.data, len(listed), _stream()))
+    if table.dtype != np.int32:
+        if table.min() < 0 or table.max() >= 1 << 31:
+            _refuse("copy_pages: a page or a number of positions is negative or too large")
+        table = table.astype(np.int32)
+    table = np.ascontiguousarray(table)
+    _check_vectors("copy_pages", k.get_device(), ())
+    _check(library().celeg_copy_pages(*sides, table.__array_interface__["data"][0], table.shape[0], _stream()))
 
 
 def keep_drafts(k: torch.Tensor, v: torch.Tensor, parents: torch.Tensor, tokens: torch.Tensor, chosen: torch.Tensor,
@@ -987,18 +987,15 @@ def keep_drafts(k: torch.Tensor, v: torch.Tensor, parents: torch.Tensor, tokens:
     name = "keep_drafts"
     sides = _cache_sides(name, k, v)
     count = min(parents.numel(), tokens.numel(), chosen.numel())
-    _vector32(name, parents, 0, "parents")
-    _vector32(name, tokens, 0, "tokens")
-    _vector32(name, chosen, 0, "chosen")
-    _vector32(name, span_begin, spans + 1, "span_begin")
-    _vector32(name, span_context, spans, "span_context")
-    _vector32(name, path, spans * max_nodes, "path")
-    _vector32(name, accepted, spans, "accepted")
-    _vector32(name, next_token, spans, "next_token")
-    _vector32(name, error_flag, 1, "error_flag")
-    if block_table.dim() != 2 or block_table.shape[0] < spans or block_table.dtype != torch.int32 or block_table.stride(1) != 1:
-        _refuse(f"{name}: a block table {tuple(block_table.shape)} of {block_table.dtype} for {spans} spans")
-    _here(name, k, v, parents, tokens, chosen, span_begin, span_context, block_table, path, accepted, next_token, error_flag)
+    _check_table(name, block_table, spans)
+    device = k.get_device()
+    if block_table.get_device() != device:
+        _refuse(f"{name}: caches on {k.device}, block table on {block_table.device}")
+    _check_vectors(name, device, (
+        ("parents", parents, 0, _I32), ("tokens", tokens, 0, _I32), ("chosen", chosen, 0, _I32),
+        ("span_begin", span_begin, spans + 1, _I32), ("span_context", span_context, spans, _I32),
+        ("path", path, spans * max_nodes, _I32), ("accepted", accepted, spans, _I32), ("next_token", next_token, spans, _I32),
+        ("error_flag", error_flag, 1, _I32)))
     _check(library().celeg_keep_drafts(
         *sides, parents.data_ptr(), tokens.data_ptr(), chosen.data_ptr(), count, span_begin.data_ptr(), span_context.data_ptr(),
         block_table.data_ptr(), block_table.stride(0), spans, max_nodes, path.data_ptr(), accepted.data_ptr(),
@@ -1018,25 +1015,24 @@ def token_logprobs(logits: torch.Tensor, rows: int, tokens: Optional[torch.Tenso
     if logits.dim() != 2 or logits.stride(1) != 1 or logits.shape[0] < rows or rows < 0:
         _refuse(f"{name}: logits {tuple(logits.shape)} with strides {logits.stride()} for {rows} rows")
     vocab = logits.shape[1]
+    vectors = []
     if logprobs is not None:
         if tokens is None:
             _refuse(f"{name}: log probabilities of no tokens")
-        _vector32(name, logprobs, rows, "logprobs", torch.float32)
-        _vector32(name, tokens, rows, "tokens")
+        vectors += (("logprobs", logprobs, rows, torch.float32), ("tokens", tokens, rows, _I32))
     if entropy is not None:
-        _vector32(name, entropy, rows, "entropy", torch.float32)
+        vectors.append(("entropy", entropy, rows, torch.float32))
     top = 0
-    if (top_logprobs is None) != (top_tokens is None):
-        _refuse(f"{name}: top_logprobs and top_tokens come together")
-    if top_tokens is not None:
+    if top_tokens is not None and top_logprobs is not None:
         if top_tokens.dim() != 2 or top_logprobs.shape != top_tokens.shape:
             _refuse(f"{name}: top_logprobs {tuple(top_logprobs.shape)} and top_tokens {tuple(top_tokens.shape)}")
         top = top_tokens.shape[1]
         if top > MAX_TOP_LOGPROBS or top > vocab:
             _refuse(f"{name}: {top} alternatives, at most {MAX_TOP_LOGPROBS} and the vocabulary of {vocab}")
-        _vector32(name, top_logprobs, rows * top, "top_logprobs", torch.float32)
-        _vector32(name, top_tokens, rows * top, "top_tokens")
-    _here(name, logits, tokens, logprobs, entropy, top_logprobs, top_tokens)
+        vectors += (("top_logprobs", top_logprobs, rows * top, torch.float32), ("top_tokens", top_tokens, rows * top, _I32))
+    elif top_tokens is not None or top_logprobs is not None:
+        _refuse(f"{name}: top_logprobs and top_tokens come together")
+    _check_vectors(name, logits.get_device(), vectors)
     _check(library().celeg_token_logprobs(
         logits.data_ptr(), logits.stride(0), rows, vocab, _ptr(tokens), _ptr(logprobs), _ptr(entropy), _ptr(top_logprobs),
         _ptr(top_tokens), top, code, _stream()))

@@ -91,6 +91,12 @@ def test_the_library_refuses_sizes():
 
     def copy(pages=5, element=4, count=1, dim=8):
         return lib.celeg_copy_pages(16, 100, 20, dim, 16, 100, 20, 8, 2, pages, 1, 4, element, moves.ctypes.data, count, None)
+    for clash in ([[0, 1, 4], [2, 1, 4]], [[0, 1, 4], [1, 2, 4]], [[3, 3, 1], [3, 4, 1]]):
+        moves = np.array(clash, dtype=np.int32)
+        assert copy(count=2) == -1 and b"another" in lib.celeg_last_error()
+    moves = np.array([[i, 4000 + i, 1] for i in range(3000)] + [[5000, 9000, 1]], dtype=np.int32)      # a table beyond the stack's
+    assert copy(pages=10000, count=3001) == -1 and b"move 3000" in lib.celeg_last_error()
+    moves = np.array([[0, 4, 1]], dtype=np.int32)
     assert copy(pages=4) == -1 and copy(element=1) == -1 and copy(dim=-1) == -1 and copy(count=-1) == -1 and copy(count=0) == 0
 
     def keep(max_nodes=4, spans=1, element=2):
