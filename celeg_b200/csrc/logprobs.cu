@@ -3,19 +3,20 @@
 //
 //   m = max x, Z = sum e^(x - m), log p(t) = x_t - m - ln Z, H = ln Z - sum e^(x - m) (x - m) / Z
 //
-// A row is one cluster of 1, 2, 4 or 8 blocks (few rows are cut so that they still fill the GPU); every thread keeps a running
-// maximum with the two sums relative to it and, in float32 arithmetic on differences x - m, loses nothing to large logits. The
-// blocks' sums meet in the first block's shared memory, added up in double in a fixed order: the same inputs give the same bits.
-// ln Z is taken as log1p of the sum without the largest logit's own 1, which is why that logit's thread is summed
-// again without it: a row whose first token has nearly all the weight keeps the digits of its small numbers.
+// A row is one cluster of 1, 2, 4 or 8 blocks (few rows are cut so that they still fill the GPU). Every thread keeps the largest
+// logit so far, where it stands, and the two sums relative to it, of differences x - m, so that large logits cost no digits.
+// The sum leaves the largest logit's own 1 out: ln Z is log1p of what is left, and a row whose first token has nearly all the
+// weight keeps the digits of its small numbers. Sums over threads and blocks are taken in double and in a fixed order: the
+// same inputs give the same bits.
 //
-// The k most likely (ties: the lowest index): a thread's largest logit is a 64-bit key (value, lowest index first); all that
-// is among the block's k largest lies with the threads whose keys are among the k largest keys, and is no smaller than the
-// smallest of these. Those threads' logits (a few hundred of them) are read again, what reaches the bound is ranked by
-// counting, and the blocks' lists are ranked the same way in the first block.
+// The k most likely (ties: the lowest index): a thread's largest logit is a 64-bit key (value, lowest index first), a group of 1 to
+// 8 threads has the largest of its threads' keys, of which there are 256 to 32, at least 2 k. All that is among the block's k
+// largest lies with the groups whose keys are among the k largest, and is no smaller than the smallest of these. Those groups'
+// logits are read again, what reaches the bound is ranked by counting, and the blocks' lists are ranked the same way in the
+// first block, where everything a block has meets.
+//
+// Over many rows the logits' bytes are what bounds it; of few rows, the chain of a block's reductions.
 #include "common.cuh"
-
-#include <cooperative_groups.h>
 
 namespace celeg_b200 {
 
@@ -23,7 +24,6 @@ constexpr int kLpThreads = 256;
 constexpr int kLpMaxTop = 128;
 constexpr int kLpPool = 1024;              // candidates of a block that are ranked at once
 constexpr int kLpMaxBlocks = 8;            // of a cluster
-constexpr int kLpUnits = 4;                // vectors a thread reads together
 constexpr float kLpLog2e = 1.4426950408889634f;
 constexpr float kLpFloor = -1.0e4f;        // differences below it count as it: e^-10000 is 0 in float32 and stays 0 times it
 
@@ -47,6 +47,11 @@ __device__ __forceinline__ LpKey lp_key(float x, int index) {
     return ((LpKey)order << 32) | (unsigned)(0x7fffffff - index);
 }
 __device__ __forceinline__ int lp_index(LpKey key) { return 0x7fffffff - (int)(unsigned)(key & 0xffffffffu); }
+__device__ __forceinline__ float lp_value(LpKey key) {
+    const unsigned order = (unsigned)(key >> 32);
+    return order == 1u ? __uint_as_float(0x7fc00000u) : __uint_as_float(order & 0x80000000u ? order & 0x7fffffffu : ~order);
+}
+constexpr unsigned kLpOrderOfMinusInf = 0x007fffffu;        // the upper half of -inf's key, above NaN's, below all numbers'
 
 __device__ __forceinline__ float lp_exp(float difference) {       // of a difference <= 0
     float e;
@@ -105,19 +110,36 @@ struct LpShare {
     __device__ __forceinline__ int edge_index(int i) const { return i < head ? i : vectors * V + i; }
 };
 
-struct LpSums { float m, z, s; };      // maximum, sum of e^(x - m), sum of e^(x - m) (x - m)
+// Of a thread's logits so far: the largest m, the sum z of e^(x - m) over all but one that is the largest (over all while none
+// has exceeded the lowest finite number, which m starts from), the sum s of e^(x - m) (x - m), the index where m stood first.
+struct LpSums {
+    float m, z, s;
+    int index;                     // -1: m has not been exceeded
+};
 
-template <int N>
-__device__ __forceinline__ bool lp_add(LpSums& a, const float* x) {
+// `index_of(e)`: where x[e] stands, rising with e.
+template <int N, typename IndexOf>
+__device__ __forceinline__ void lp_add(LpSums& a, const float (&x)[N], IndexOf index_of) {
     float top = x[0];
 #pragma unroll
     for (int i = 1; i < N; ++i) top = fmaxf(top, x[i]);
-    const bool grown = top > a.m;
-    if (grown) {
-        const float d = lp_difference(a.m, top), f = lp_exp(d);
-        a.s = f * fmaf(d, a.z, a.s);
-        a.z *= f;
+    if (top > a.m) {
+        const float d = lp_difference(a.m, top), f = lp_exp(d), all = a.z + (a.index >= 0 ? 1.0f : 0.0f);
+        a.s = f * fmaf(d, all, a.s);
+        a.z = f * all;
         a.m = top;
+        int first = 0;
+#pragma unroll
+        for (int i = N - 1; i >= 0; --i) first = x[i] == top ? i : first;
+        a.index = index_of(first);
+        // all but the first that is the largest, so that its 1 is never part of the sum
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float di = lp_difference(x[i], top), e = i == first ? 0.0f : lp_exp(di);
+            a.z += e;
+            a.s = fmaf(e, di, a.s);
+        }
+        return;
     }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -125,28 +147,27 @@ __device__ __forceinline__ bool lp_add(LpSums& a, const float* x) {
         a.z += e;
         a.s = fmaf(e, d, a.s);
     }
-    return grown;
 }
 
 struct LpShared {
-    LpKey keys[kLpThreads];                    // every thread's largest
+    LpKey keys[kLpThreads];                    // the groups' largest
     LpKey pool[kLpPool];
-    LpKey lists[kLpMaxBlocks][kLpMaxTop];      // of the cluster's blocks (the first block's copy is the one used)
+    LpKey list[kLpMaxTop];                     // of this block
+    LpKey lists[kLpMaxBlocks * kLpMaxTop];     // of the cluster's blocks, in the first one
     double z[kLpMaxBlocks], s[kLpMaxBlocks];
     float m[kLpMaxBlocks];
     LpKey largest[kLpMaxBlocks];
     double warp_z[8], warp_s[8];
     LpKey warp_key[8];
     float warp_m[8];
-    int selected[kLpThreads];
-    int pooled, nan_seen;
-    float row_max;
+    int selected[kLpMaxTop];
+    int pooled;
+    float row_max, log_z;
     LpKey bound;
 };
 
-__device__ __forceinline__ LpKey lp_key_max(LpKey key) {
-#pragma unroll
-    for (int lanes = 16; lanes > 0; lanes >>= 1) {
+__device__ __forceinline__ LpKey lp_key_max(LpKey key, int from = 16) {
+    for (int lanes = from; lanes > 0; lanes >>= 1) {
         const LpKey other = __shfl_xor_sync(0xffffffffu, key, lanes);
         key = other > key ? other : key;
     }
@@ -159,60 +180,93 @@ __device__ __forceinline__ double lp_warp_sum(double v) {
     return v;
 }
 
-// A warp reads the logits of thread `owner` again: visit(index, value).
-template <typename A, typename Visit>
-__device__ __forceinline__ void lp_reread(const LpShare<A>& share, int owner, int lane, Visit visit) {
-    constexpr int V = LpVector<A>::kSize;
-    for (int i = owner + lane * kLpThreads; i < share.count; i += 32 * kLpThreads) {
-        float x[V];
-        const int index = share.vector_index(i);
-        LpVector<A>::load(share.row + index, x);
-#pragma unroll
-        for (int e = 0; e < V; ++e) visit(index + e, x[e]);
+// How many of `keys` (`count` of them, a multiple of 2) are above `key`.
+__device__ __forceinline__ int lp_rank(const LpKey* keys, int count, LpKey key) {
+    int rank = 0;
+#pragma unroll 4
+    for (int i = 0; i < count; i += 2) {
+        const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(keys + i);
+        rank += (two.x > key) + (two.y > key);
     }
-    if (lane == 0 && owner < share.edge) {
-        const int index = share.edge_index(owner);
-        visit(index, to_float(share.row[index]));
+    return rank;
+}
+
+// The logits of `chosen` groups of 2^shift threads, read again by all threads: visit(index, value).
+template <typename A, typename Visit>
+__device__ __forceinline__ void lp_reread(const LpShared& sh, const LpShare<A>& share, int chosen, int shift, Visit visit) {
+    constexpr int V = LpVector<A>::kSize;
+    const int rounds = (share.count + kLpThreads - 1) / kLpThreads, per_group = rounds << shift;
+    for (int item0 = threadIdx.x; item0 < chosen * per_group; item0 += 4 * kLpThreads) {
+        float x[4][V];
+        int index[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int item = item0 + u * kLpThreads, group = item / per_group, rest = item % per_group;
+            index[u] = -1;
+            if (item >= chosen * per_group) continue;
+            const int i = (sh.selected[group] << shift) + (rest & ((1 << shift) - 1)) + (rest >> shift) * kLpThreads;
+            if (i >= share.count) continue;
+            index[u] = share.vector_index(i);
+            LpVector<A>::load(share.row + index[u], x[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (index[u] < 0) continue;
+#pragma unroll
+            for (int e = 0; e < V; ++e) visit(index[u] + e, x[u][e]);
+        }
+    }
+    for (int item = threadIdx.x; item < chosen << shift; item += kLpThreads) {
+        const int owner = (sh.selected[item >> shift] << shift) + (item & ((1 << shift) - 1));
+        if (owner < share.edge) {
+            const int index = share.edge_index(owner);
+            visit(index, to_float(share.row[index]));
+        }
     }
 }
 
-// The `top` largest of the block's logits into `list`, largest first; 0 where there are fewer.
+// The `top` largest of the block's logits into sh.list, largest first; 0 where there are fewer.
 template <typename A>
-__device__ __forceinline__ void lp_block_top(LpShared& sh, const LpShare<A>& share, const LpKey mine, const int top, LpKey* list) {
+__device__ __forceinline__ void lp_block_top(LpShared& sh, const LpShare<A>& share, const LpKey mine, const int top) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    sh.keys[tid] = mine;
+    // 32 groups of 8 threads for up to 16, ..., 256 of one for more than 64
+    const int shift = top <= 16 ? 3 : top <= 32 ? 2 : top <= 64 ? 1 : 0, groups = kLpThreads >> shift;
+    const LpKey group_key = shift > 0 ? lp_key_max(mine, 1 << (shift - 1)) : mine;
+    if ((tid & ((1 << shift) - 1)) == 0) sh.keys[tid >> shift] = group_key;
     if (tid == 0) sh.pooled = 0;
-    if (tid < top) list[tid] = 0;
+    if (tid < top) sh.list[tid] = 0;
     __syncthreads();
+    bool chosen_one = false;
+    LpKey key = 0;
     int rank = 0;
-    for (int i = 0; i < kLpThreads; i += 2) {
-        const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(&sh.keys[i]);
-        rank += (two.x > mine) + (two.y > mine);
+    if (tid < groups) {
+        key = sh.keys[tid];
+        rank = lp_rank(sh.keys, groups, key);
+        // (keys of groups without logits are 0 and rank behind all others; they have nothing to read)
+        chosen_one = rank < top && key != 0;
+        if (chosen_one) sh.selected[rank] = tid;
     }
-    // (keys of threads without logits are 0 and rank behind all others; they have nothing to read)
-    if (rank < top && mine != 0) sh.selected[rank] = tid;
-    if (rank >= top || mine == 0) rank = -1;
-    const int chosen = __syncthreads_count(rank >= 0);
-    if (rank == chosen - 1 && chosen > 0) sh.bound = mine;
+    const int chosen = __syncthreads_count(chosen_one);
+    if (chosen_one && rank == chosen - 1) sh.bound = key;
     __syncthreads();
     if (chosen == 0) return;
-    LpKey bound = chosen == top ? sh.bound : 0;
-    for (int w = warp; w < chosen; w += kLpThreads / 32)
-        lp_reread<A>(share, sh.selected[w], lane, [&](int index, float x) {
-            const LpKey key = lp_key(x, index);
-            if (key >= bound) {
-                const int at = atomicAdd(&sh.pooled, 1);
-                if (at < kLpPool) sh.pool[at] = key;
-            }
-        });
+    const LpKey bound = chosen == top ? sh.bound : 0;
+    lp_reread<A>(sh, share, chosen, shift, [&](int index, float x) {
+        const LpKey k = lp_key(x, index);
+        if (k >= bound) {
+            const int at = atomicAdd(&sh.pooled, 1);
+            if (at < kLpPool) sh.pool[at] = k;
+        }
+    });
     __syncthreads();
     const int pooled = sh.pooled;
     if (pooled <= kLpPool) {
+        if (tid == 0 && (pooled & 1)) sh.pool[pooled] = 0;
+        __syncthreads();
         for (int i = tid; i < pooled; i += kLpThreads) {
-            const LpKey key = sh.pool[i];
-            int above = 0;
-            for (int j = 0; j < pooled; ++j) above += sh.pool[j] > key;
-            if (above < top) list[above] = key;
+            const LpKey k = sh.pool[i];
+            const int above = lp_rank(sh.pool, (pooled + 1) & ~1, k);
+            if (above < top) sh.list[above] = k;
         }
         __syncthreads();
         return;
@@ -222,212 +276,188 @@ __device__ __forceinline__ void lp_block_top(LpShared& sh, const LpShare<A>& sha
     LpKey before = ~0ull;
     for (int n = 0; n < top; ++n) {
         LpKey best = 0;
-        for (int w = warp; w < chosen; w += kLpThreads / 32)
-            lp_reread<A>(share, sh.selected[w], lane, [&](int index, float x) {
-                const LpKey key = lp_key(x, index);
-                if (key < before && key > best) best = key;
-            });
+        lp_reread<A>(sh, share, chosen, shift, [&](int index, float x) {
+            const LpKey k = lp_key(x, index);
+            if (k < before && k > best) best = k;
+        });
         best = lp_key_max(best);
         if (lane == 0) sh.warp_key[warp] = best;
         __syncthreads();
         for (int w = 0; w < kLpThreads / 32; ++w) best = sh.warp_key[w] > best ? sh.warp_key[w] : best;
         before = best;
-        if (tid == 0) list[n] = best;
+        if (tid == 0) sh.list[n] = best;
         __syncthreads();
     }
 }
 
+__device__ __forceinline__ unsigned lp_first_block(const void* shared) {       // the same place in the cluster's first block
+    unsigned address;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;\n" : "=r"(address) : "r"((unsigned)__cvta_generic_to_shared(shared)));
+    return address;
+}
+__device__ __forceinline__ void lp_give(unsigned address, unsigned long long value) {
+    asm volatile("st.shared::cluster.b64 [%0], %1;\n" ::"r"(address), "l"(value) : "memory");
+}
+
 template <typename A>
-__global__ void __launch_bounds__(kLpThreads) token_logprobs_kernel(const LogprobParams p, const int blocks) {
-    namespace cg = cooperative_groups;
-    constexpr int V = LpVector<A>::kSize;
+__global__ void __launch_bounds__(kLpThreads, 3) token_logprobs_kernel(const LogprobParams p, const int blocks) {
+    constexpr int V = LpVector<A>::kSize, kUnits = 16 / V;      // 16 logits a thread at a time, the next 16 under way
     __shared__ __align__(16) LpShared sh;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = blockIdx.x % blocks;
     const long long at = blockIdx.x / blocks;
+    chain_release();
+    chain_wait();
     const LpShare<A> share(p, at, rank, blocks);
     if (blocks > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
 
     // ---- the pass over the logits
-    LpSums mine = {-3.402823466e38f, 0.0f, 0.0f};
-    int top_vector = -1;                        // the first vector group in which the thread's maximum stood
-    for (int i0 = tid; i0 < share.count; i0 += kLpUnits * kLpThreads) {
-        float x[kLpUnits * V];
-        if (i0 + (kLpUnits - 1) * kLpThreads < share.count) {
-#pragma unroll
-            for (int u = 0; u < kLpUnits; ++u) LpVector<A>::load(share.row + share.vector_index(i0 + u * kLpThreads), x + u * V);
-            if (lp_add<kLpUnits * V>(mine, x)) top_vector = i0;
-        } else {
-            for (int i = i0; i < share.count; i += kLpThreads) {
-                LpVector<A>::load(share.row + share.vector_index(i), x);
-                if (lp_add<V>(mine, x)) top_vector = i0;
-            }
-        }
-    }
-    bool top_edge = false;
-    if (tid < share.edge) {
-        const float x = to_float(share.row[share.edge_index(tid)]);
-        top_edge = lp_add<1>(mine, &x);
-    }
-    // the thread's key: the lowest index at which its maximum stands
-    LpKey key = 0;
+    LpSums mine = {-3.402823466e38f, 0.0f, 0.0f, -1};
     {
-        int index = 0x7fffffff;
-        if (top_vector >= 0)
-            for (int u = kLpUnits - 1; u >= 0; --u) {
-                const int i = top_vector + u * kLpThreads;
-                if (i >= share.count) continue;
-                float x[V];
-                LpVector<A>::load(share.row + share.vector_index(i), x);
+        float next[kUnits][V];
+        auto load = [&](int i0) {
 #pragma unroll
-                for (int e = V - 1; e >= 0; --e)
-                    if (x[e] == mine.m) index = share.vector_index(i) + e;
-            }
-        if (tid < share.edge) {
-            const int e = share.edge_index(tid);
-            if (top_edge || (to_float(share.row[e]) == mine.m && e < index)) index = e;
+            for (int u = 0; u < kUnits; ++u) LpVector<A>::load(share.row + share.vector_index(i0 + u * kLpThreads), next[u]);
+        };
+        const int whole = share.count - (kUnits - 1) * kLpThreads;      // i0 below it: all units are there
+        int i0 = tid;
+        if (i0 < whole) load(i0);
+        for (; i0 < whole; i0 += kUnits * kLpThreads) {
+            float x[kUnits * V];
+#pragma unroll
+            for (int u = 0; u < kUnits; ++u)
+#pragma unroll
+                for (int e = 0; e < V; ++e) x[u * V + e] = next[u][e];
+            if (i0 + kUnits * kLpThreads < whole) load(i0 + kUnits * kLpThreads);
+            lp_add(mine, x, [&](int e) { return share.vector_index(i0 + e / V * kLpThreads) + e % V; });
         }
-        if (index != 0x7fffffff) {
-            key = lp_key(mine.m, index);
-        } else if (tid < share.count || tid < share.edge) {
-            // nothing above the lowest finite number: the thread's lowest index stands for its logits (-inf, NaN or that number)
-            key = 1;
+        for (; i0 < share.count; i0 += kLpThreads) {
+            float x[V];
+            LpVector<A>::load(share.row + share.vector_index(i0), x);
+            lp_add(mine, x, [&](int e) { return share.vector_index(i0) + e; });
         }
     }
-    if (key == 1) {
-        LpKey best = 0;
+    if (tid < share.edge) {
+        const int index = share.edge_index(tid);
+        const float x[1] = {to_float(share.row[index])};
+        if (x[0] == mine.m && index < mine.index) mine.index = index;      // (as large, and before all whole vectors)
+        lp_add(mine, x, [&](int) { return index; });
+    }
+    LpKey key = mine.index >= 0 ? lp_key(mine.m, mine.index) : 0;
+    if (mine.index < 0 && (tid < share.count || tid < share.edge)) {
+        // nothing above the lowest finite number: -inf, NaN or that number
         for (int i = tid; i < share.count; i += kLpThreads) {
             float x[V];
             LpVector<A>::load(share.row + share.vector_index(i), x);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 const LpKey k = lp_key(x[e], share.vector_index(i) + e);
-                best = k > best ? k : best;
+                key = k > key ? k : key;
             }
         }
         if (tid < share.edge) {
             const LpKey k = lp_key(to_float(share.row[share.edge_index(tid)]), share.edge_index(tid));
-            best = k > best ? k : best;
+            key = k > key ? k : key;
         }
-        key = best;
     }
 
-    // ---- the block's largest logit, and its sums relative to it
+    // ---- the block's largest logit, and its sums relative to it, without that logit
+    LpKey block_best;
     {
         const LpKey best = lp_key_max(key);
-        if (lane == 0) sh.warp_key[warp] = best;
+        float m = warp_max(mine.m);
+        if (lane == 0) {
+            sh.warp_key[warp] = best;
+            sh.warp_m[warp] = m;
+        }
         __syncthreads();
-        LpKey block_best = sh.warp_key[0];
+        block_best = sh.warp_key[0];
         for (int w = 1; w < kLpThreads / 32; ++w) block_best = sh.warp_key[w] > block_best ? sh.warp_key[w] : block_best;
-        float m = mine.m;
-        m = warp_max(m);
-        if (lane == 0) sh.warp_m[warp] = m;
-        __syncthreads();
         for (int w = 0; w < kLpThreads / 32; ++w) m = fmaxf(m, sh.warp_m[w]);
-        float z = mine.z, s = mine.s;
-        if (key == block_best) z = s = 0.0f;           // (summed again below, without the largest itself)
+        // a thread's largest is a 1 of its own sum unless it is the block's (while nothing exceeded the start, it is in the sum)
+        const float own = mine.index >= 0 ? 1.0f : 0.0f;
+        float z = mine.z + own;
+        if (key == block_best && key >> 32 > kLpOrderOfMinusInf) z = mine.index >= 0 ? mine.z : mine.z - 1.0f;
         const float d = lp_difference(mine.m, m), f = expf(d);
-        const double wz = lp_warp_sum((double)z * f), ws = lp_warp_sum((double)(f * fmaf(d, z, s)));
+        const double wz = lp_warp_sum((double)(z * f)), ws = lp_warp_sum((double)(f * fmaf(d, z, mine.s)));
         if (lane == 0) {
             sh.warp_z[warp] = wz;
             sh.warp_s[warp] = ws;
         }
-        if (key == block_best) sh.selected[0] = tid;
         // (another block's shared memory may be written once that block has begun)
         if (blocks > 1) asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
         __syncthreads();
-        if (warp == 0) {
-            const int skip = lp_index(block_best);
-            float rz = 0.0f, rs = 0.0f;
-            if (block_best != 0)
-                lp_reread<A>(share, sh.selected[0], lane, [&](int index, float x) {
-                    if (index == skip && x == m) return;
-                    const float dx = lp_difference(x, m), e = lp_exp(dx);
-                    rz += e;
-                    rs = fmaf(e, dx, rs);
-                });
-            double tz = lp_warp_sum((double)rz), ts = lp_warp_sum((double)rs);
-            if (lane == 0) {
-                for (int w = 0; w < kLpThreads / 32; ++w) tz += sh.warp_z[w], ts += sh.warp_s[w];
-                // (without the largest: its 1 is added where the blocks meet)
-                cg::cluster_group cluster = cg::this_cluster();
-                LpShared* first = blocks > 1 ? cluster.map_shared_rank(&sh, 0) : &sh;
-                first->z[rank] = tz;
-                first->s[rank] = ts;
-                first->m[rank] = m;
-                first->largest[rank] = block_best;
-            }
+        if (tid == 0) {
+            double tz = 0.0, ts = 0.0;
+            for (int w = 0; w < kLpThreads / 32; ++w) tz += sh.warp_z[w], ts += sh.warp_s[w];
+            lp_give(lp_first_block(&sh.z[rank]), (unsigned long long)__double_as_longlong(tz));
+            lp_give(lp_first_block(&sh.s[rank]), (unsigned long long)__double_as_longlong(ts));
+            lp_give(lp_first_block(&sh.largest[rank]), block_best);
+            asm volatile("st.shared::cluster.f32 [%0], %1;\n" ::"r"(lp_first_block(&sh.m[rank])), "f"(m) : "memory");
         }
+    }
+    if (p.top > 1) {
+        lp_block_top<A>(sh, share, key, p.top);
+        if (tid < p.top) lp_give(lp_first_block(&sh.lists[rank * p.top + tid]), sh.list[tid]);
+    }
+    if (blocks > 1)
+        asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+    else
         __syncthreads();
-    }
-    if (p.top > 0) {
-        lp_block_top<A>(sh, share, key, p.top, sh.lists[blocks > 1 ? kLpMaxBlocks - 1 : 0]);
-    }
-    if (blocks > 1) {
-        cg::cluster_group cluster = cg::this_cluster();
-        cluster.sync();
-        // (the lists of all blocks go to the first one; its own list lies at its last place until then)
-        if (p.top > 0) {
-            LpKey* to = cluster.map_shared_rank(&sh, 0)->pool + rank * kLpMaxTop;
-            const LpKey value = tid < p.top ? sh.lists[kLpMaxBlocks - 1][tid] : 0;
-            if (tid < p.top) to[tid] = value;
-        }
-        cluster.sync();
-        if (rank != 0) return;
-    }
+    if (rank != 0) return;
 
     // ---- the first block puts the row together
-    if (tid == 0) {
-        float m = sh.m[0];
-        LpKey largest = sh.largest[0];
-        for (int b = 1; b < blocks; ++b) {
-            m = fmaxf(m, sh.m[b]);
-            largest = sh.largest[b] > largest ? sh.largest[b] : largest;
+    if (warp == 0) {
+        const bool one = lane < blocks;
+        const LpKey own = one ? sh.largest[lane] : 0, largest = lp_key_max(own);
+        const float own_m = one ? sh.m[lane] : -3.402823466e38f, m = warp_max(own_m);
+        // a block's largest is a 1 of its own sum, unless it is the row's
+        const double z_own = one ? sh.z[lane] + (own != largest && own >> 32 > kLpOrderOfMinusInf ? 1.0 : 0.0) : 0.0;
+        const float d = lp_difference(own_m, m), f = expf(d);
+        const double z = lp_warp_sum(z_own * f), s = lp_warp_sum(one ? f * (sh.s[lane] + d * z_own) : 0.0);
+        if (lane == 0) {
+            // a row without a logit above -inf has no distribution, nor has one with a logit of inf
+            const bool none = (unsigned)(largest >> 32) <= kLpOrderOfMinusInf || m == INFINITY;
+            const float log_z = none ? __uint_as_float(0x7fc00000u) : log1pf((float)z);
+            if (p.entropy) p.entropy[at] = log_z - (float)(s / (1.0 + z));
+            if (p.logprobs) {
+                const int token = p.tokens[at];
+                const bool inside = token >= 0 && token < p.vocab;
+                p.logprobs[at] = inside ? to_float(share.row[token]) - m - log_z : __uint_as_float(0x7fc00000u);
+            }
+            sh.row_max = m;
+            sh.log_z = log_z;
+            if (p.top == 1) {
+                p.top_tokens[at] = lp_index(largest);
+                p.top_logprobs[at] = lp_value(largest) - m - log_z;
+            }
         }
-        double z = 0.0, s = 0.0;
-        for (int b = 0; b < blocks; ++b) {
-            // a block's largest is a 1 of its own sum, unless it is the row's largest
-            const double own = sh.largest[b] == largest ? 0.0 : (sh.largest[b] >> 32 > 0x007fffffu ? 1.0 : 0.0);
-            const double d = (double)lp_difference(sh.m[b], m), f = exp(d), bz = sh.z[b] + own;
-            z += bz * f;
-            s += f * (sh.s[b] + d * bz);
-        }
-        // a row without a logit above -inf has no distribution, nor has one with a logit of inf
-        const bool none = (unsigned)(largest >> 32) <= 0x007fffffu || m == INFINITY;
-        const double log_z = none ? nan("") : log1p(z);
-        if (p.entropy) p.entropy[at] = (float)(log_z - s / (1.0 + z));
-        if (p.logprobs) {
-            const int token = p.tokens[at];
-            const bool inside = token >= 0 && token < p.vocab;
-            p.logprobs[at] = inside ? (float)((double)to_float(share.row[token]) - (double)m - log_z) : nanf("");
-        }
-        sh.row_max = m;
-        sh.z[0] = log_z;
     }
-    if (p.top == 0) return;
+    if (p.top <= 1) return;
     __syncthreads();
-    const double log_z = sh.z[0];
-    const float m = sh.row_max;
-    const LpKey* lists = blocks > 1 ? sh.pool : sh.lists[0];
-    for (int i = tid; i < blocks * p.top; i += kLpThreads) {
-        const LpKey k = lists[(i / p.top) * kLpMaxTop + i % p.top];
+    const float log_z = sh.log_z, m = sh.row_max;
+    const int entries = blocks * p.top;
+    for (int i = tid; i < entries; i += kLpThreads) {
+        const LpKey k = sh.lists[i];
         if (k == 0) continue;
         int above = i % p.top;                          // (its own list is in order)
-        if (blocks > 1)
+        if (blocks > 1 && entries <= 256 && entries % 2 == 0) {
+            above = lp_rank(sh.lists, entries, k);
+        } else if (blocks > 1) {
             for (int b = 0; b < blocks; ++b) {
                 if (b == i / p.top) continue;
                 // how many of another list are above it: lists fall
                 int low = 0, high = p.top;
                 while (low < high) {
                     const int middle = (low + high) / 2;
-                    if (lists[b * kLpMaxTop + middle] > k) low = middle + 1; else high = middle;
+                    if (sh.lists[b * p.top + middle] > k) low = middle + 1; else high = middle;
                 }
                 above += low;
             }
+        }
         if (above >= p.top) continue;
-        const int index = lp_index(k);
-        p.top_tokens[at * p.top + above] = index;
-        p.top_logprobs[at * p.top + above] = (float)((double)to_float(share.row[index]) - (double)m - log_z);
+        p.top_tokens[at * p.top + above] = lp_index(k);
+        p.top_logprobs[at * p.top + above] = lp_value(k) - m - log_z;
     }
 }
 
@@ -437,13 +467,13 @@ static int launch_logprobs(const LogprobParams& p, int blocks, cudaStream_t stre
     config.gridDim = dim3((unsigned)((long long)p.rows * blocks));
     config.blockDim = dim3(kLpThreads);
     config.stream = stream;
-    cudaLaunchAttribute attribute[1];
-    attribute[0].id = cudaLaunchAttributeClusterDimension;
-    attribute[0].val.clusterDim.x = blocks;
-    attribute[0].val.clusterDim.y = 1;
-    attribute[0].val.clusterDim.z = 1;
-    config.attrs = attribute;
-    config.numAttrs = blocks > 1 ? 1 : 0;
+    cudaLaunchAttribute attributes[2];
+    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[0].val.programmaticStreamSerializationAllowed = chaining_enabled() ? 1 : 0;
+    attributes[1].id = cudaLaunchAttributeClusterDimension;
+    attributes[1].val.clusterDim = {(unsigned)blocks, 1, 1};
+    config.attrs = attributes;
+    config.numAttrs = blocks > 1 ? 2 : 1;
     const cudaError_t status = cudaLaunchKernelEx(&config, token_logprobs_kernel<A>, p, blocks);
     CELEG_REQUIRE(status == cudaSuccess, "token_logprobs: %s", cudaGetErrorString(status));
     return check_launch("token_logprobs");
