@@ -686,10 +686,23 @@ bool tree_tcgen05_takes(const TreeParams& p) {
 // Two teams' rows a tile where one tile of 128 does not hold them: the same keys would be read for every tile.
 static bool tree_paired(const TreeParams& p) { return p.max_nodes * p.group > kTtM; }
 
+// The kernel may have its shared memory: said once a device (a call of its own costs a small launch a tenth of its time).
+template <int D, bool PAIRED>
+static cudaError_t allow_shared_memory() {
+    static std::atomic<unsigned long long> said;
+    int device = 0;
+    cudaError_t status = cudaGetDevice(&device);
+    if (status != cudaSuccess || (device < 64 && (said.load(std::memory_order_relaxed) >> device & 1))) return status;
+    status = cudaFuncSetAttribute(attention_tree_tcgen05_kernel<D, PAIRED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  (int)TtLayout<D, PAIRED>::kSmemBytes);
+    if (status == cudaSuccess && device < 64) said.fetch_or(1ull << device, std::memory_order_relaxed);
+    return status;
+}
+
 template <int D, bool PAIRED>
 static cudaError_t tree_config(cudaLaunchConfig_t& config, cudaLaunchAttribute (&attributes)[2], int cluster) {
     constexpr unsigned smem = TtLayout<D, PAIRED>::kSmemBytes;
-    const cudaError_t status = cudaFuncSetAttribute(attention_tree_tcgen05_kernel<D, PAIRED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    const cudaError_t status = allow_shared_memory<D, PAIRED>();
     config.blockDim = dim3(kTtThreads);
     config.dynamicSmemBytes = smem;
     attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -862,7 +862,8 @@ _I32 = torch.int32
 
 def _check_vectors(operator: str, device: int, vectors) -> None:
     """``vectors``: (name, tensor, least number of elements, type) of contiguous tensors on CUDA device ``device``, which has to
-    be the current one: the launch goes to its current stream."""
+    be the current one: the launch goes to its current stream. (The wrappers below that small steps call ask the same in one
+    expression first, which takes a third of the time, and come here for the name of what is wrong.)"""
     for name, tensor, elements, dtype in vectors:
         if tensor.dtype is not dtype or tensor.numel() < elements or not tensor.is_contiguous():
             _refuse(f"{operator}: {name} must be a contiguous tensor of {dtype} with at least {elements} elements, got "
@@ -874,7 +875,8 @@ def _check_vectors(operator: str, device: int, vectors) -> None:
 
 
 def _check_table(operator: str, table: torch.Tensor, spans: int) -> None:
-    if table.dim() != 2 or table.shape[0] < spans or table.dtype is not _I32 or table.stride(1) != 1:
+    shape = table.shape
+    if len(shape) != 2 or shape[0] < spans or table.dtype is not _I32 or table.stride(1) != 1:
         _refuse(f"{operator}: a block table {tuple(table.shape)} of {table.dtype} for {spans} spans")
 
 
@@ -905,32 +907,38 @@ def attention_tree(q: torch.Tensor, q_row_stride: int, out: torch.Tensor, k_cach
     code = dtype_code(dtype)
     if k_cache.dtype is not dtype or v_cache.dtype is not dtype:
         _refuse(f"{name}: q {dtype}, caches {k_cache.dtype} and {v_cache.dtype}")
-    strides = k_cache.stride()
-    shape = k_cache.shape
+    strides, shape = k_cache.stride(), k_cache.shape
     if (shape[1:] != (kv_heads, page_tokens, head_dim) or strides[1:] != (page_tokens * head_dim, head_dim, 1) or v_cache.shape != shape
             or v_cache.stride() != strides):
         _refuse(f"{name}: caches [pages, kv_heads, page_tokens, head_dim] with pages {(kv_heads, page_tokens, head_dim)} in one piece are "
                 f"needed, got {tuple(shape)} and {tuple(v_cache.shape)} with strides {strides} and {v_cache.stride()}")
-    if (q.dim() != 2 or q.stride(1) != 1 or q.shape[0] < tokens or q.shape[1] < q_heads * head_dim
-            or (tokens > 1 and q.stride(0) != q_row_stride)):
-        _refuse(f"{name}: q {tuple(q.shape)} with strides {q.stride()} does not hold {tokens} rows of {q_heads} x {head_dim}, {q_row_stride} apart")
-    if ancestors.dim() != 2 or ancestors.shape[0] < tokens:
-        _refuse(f"{name}: ancestors {tuple(ancestors.shape)} for {tokens} tokens")
+    q_shape, q_strides, masks = q.shape, q.stride(), ancestors.shape
+    if (len(q_shape) != 2 or q_strides[1] != 1 or q_shape[0] < tokens or q_shape[1] < q_heads * head_dim
+            or (tokens > 1 and q_strides[0] != q_row_stride)):
+        _refuse(f"{name}: q {tuple(q_shape)} with strides {q_strides} does not hold {tokens} rows of {q_heads} x {head_dim}, {q_row_stride} apart")
+    if len(masks) != 2 or masks[0] < tokens:
+        _refuse(f"{name}: ancestors {tuple(masks)} for {tokens} tokens")
     _check_table(name, block_table, spans)
     device = q.get_device()
-    vectors = [("out", out, tokens * q_heads * head_dim, dtype), ("positions", positions, tokens, _I32),
-               ("span_begin", span_begin, spans + 1, _I32), ("span_context", span_context, spans, _I32),
-               ("ancestors", ancestors, 0, _I32), ("error_flag", error_flag, 1, _I32)]
-    if sinks is not None:
-        vectors.append(("sinks", sinks, q_heads, torch.float32))
-    if scratch is not None:
-        vectors.append(("scratch", scratch, 0, torch.float32))
     if k_cache.get_device() != device or v_cache.get_device() != device or block_table.get_device() != device:
         _refuse(f"{name}: q on {q.device}, caches on {k_cache.device} and {v_cache.device}, block table on {block_table.device}")
-    _check_vectors(name, device, vectors)
+    if not (positions.dtype is span_begin.dtype is span_context.dtype is ancestors.dtype is error_flag.dtype is _I32 and out.dtype is dtype
+            and positions.is_contiguous() and span_begin.is_contiguous() and span_context.is_contiguous() and ancestors.is_contiguous()
+            and out.is_contiguous() and out.numel() >= tokens * q_heads * head_dim and positions.numel() >= tokens
+            and span_begin.numel() > spans and span_context.numel() >= spans and error_flag.numel() >= 1
+            and device >= 0 and positions.get_device() == span_begin.get_device() == span_context.get_device() == ancestors.get_device()
+            == error_flag.get_device() == out.get_device() == device == torch._C._cuda_getDevice()):
+        _check_vectors(name, device, (
+            ("out", out, tokens * q_heads * head_dim, dtype), ("positions", positions, tokens, _I32),
+            ("span_begin", span_begin, spans + 1, _I32), ("span_context", span_context, spans, _I32),
+            ("ancestors", ancestors, 0, _I32), ("error_flag", error_flag, 1, _I32)))
+    if sinks is not None:
+        _check_vectors(name, device, (("sinks", sinks, q_heads, torch.float32),))
+    if scratch is not None and (scratch.dtype is not torch.float32 or not scratch.is_contiguous() or scratch.get_device() != device):
+        _check_vectors(name, device, (("scratch", scratch, 0, torch.float32),))
     _check(library().celeg_attention_tree(
         q.data_ptr(), q_row_stride, out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), strides[0], shape[0],
-        positions.data_ptr(), span_begin.data_ptr(), span_context.data_ptr(), ancestors.data_ptr(), ancestors.shape[1],
+        positions.data_ptr(), span_begin.data_ptr(), span_context.data_ptr(), ancestors.data_ptr(), masks[1],
         block_table.data_ptr(), block_table.stride(0), tokens, spans, max_nodes, max_keys, q_heads, kv_heads, head_dim,
         page_tokens, int(window or 0), scale, _ptr(sinks), float(softcap or 0.0), _ptr(scratch),
         scratch.numel() if scratch is not None else 0, error_flag.data_ptr(), code, _stream()))
@@ -991,11 +999,20 @@ def keep_drafts(k: torch.Tensor, v: torch.Tensor, parents: torch.Tensor, tokens:
     device = k.get_device()
     if block_table.get_device() != device:
         _refuse(f"{name}: caches on {k.device}, block table on {block_table.device}")
-    _check_vectors(name, device, (
-        ("parents", parents, 0, _I32), ("tokens", tokens, 0, _I32), ("chosen", chosen, 0, _I32),
-        ("span_begin", span_begin, spans + 1, _I32), ("span_context", span_context, spans, _I32),
-        ("path", path, spans * max_nodes, _I32), ("accepted", accepted, spans, _I32), ("next_token", next_token, spans, _I32),
-        ("error_flag", error_flag, 1, _I32)))
+    if not (parents.dtype is tokens.dtype is chosen.dtype is span_begin.dtype is span_context.dtype is path.dtype is accepted.dtype
+            is next_token.dtype is error_flag.dtype is _I32
+            and parents.is_contiguous() and tokens.is_contiguous() and chosen.is_contiguous() and span_begin.is_contiguous()
+            and span_context.is_contiguous() and path.is_contiguous() and accepted.is_contiguous() and next_token.is_contiguous()
+            and span_begin.numel() > spans and span_context.numel() >= spans and path.numel() >= spans * max_nodes
+            and accepted.numel() >= spans and next_token.numel() >= spans and error_flag.numel() >= 1
+            and device >= 0 and parents.get_device() == tokens.get_device() == chosen.get_device() == span_begin.get_device()
+            == span_context.get_device() == path.get_device() == accepted.get_device() == next_token.get_device()
+            == error_flag.get_device() == device == torch._C._cuda_getDevice()):
+        _check_vectors(name, device, (
+            ("parents", parents, 0, _I32), ("tokens", tokens, 0, _I32), ("chosen", chosen, 0, _I32),
+            ("span_begin", span_begin, spans + 1, _I32), ("span_context", span_context, spans, _I32),
+            ("path", path, spans * max_nodes, _I32), ("accepted", accepted, spans, _I32), ("next_token", next_token, spans, _I32),
+            ("error_flag", error_flag, 1, _I32)))
     _check(library().celeg_keep_drafts(
         *sides, parents.data_ptr(), tokens.data_ptr(), chosen.data_ptr(), count, span_begin.data_ptr(), span_context.data_ptr(),
         block_table.data_ptr(), block_table.stride(0), spans, max_nodes, path.data_ptr(), accepted.data_ptr(),
