@@ -14,6 +14,7 @@ _LAZY = {
     "SchedulerPolicy": ("celeg_b200.engine.scheduler", "SchedulerPolicy"),
     "SamplingParams": ("celeg_b200.sampling.params", "SamplingParams"),
     "KernelOptions": ("celeg_b200.parts.options", "KernelOptions"),
+    "TokenScores": ("celeg_b200.engine.engine", "TokenScores"),
     "StepEntry": ("celeg_b200.engine.step", "StepEntry"),
     "load_model": ("celeg_b200.engine.loading", "load_model"),
     "write_random_model": ("celeg_b200.weights.random_init", "write_random_model"),

@@ -12,6 +12,10 @@ Two kinds of holdings, both decided by what the model's mixers ask for:
   all such layers of one request; a slot is cleared when a request takes it (celeg zeroes the
   conv state at reset: src/backend/cpu/model_state.cpp:395-397).
 
+A request can be forked (:meth:`CacheManager.fork`): the new one holds the same full pages, which nobody writes any
+more, and a copy of the last page if that is partly filled; a page goes back to its pool when its last holder gives
+it back.
+
 Everything a request holds is given back in one place, :meth:`CacheManager.close`, as celeg
 does in ``finish_request_locked`` (src/backend/cuda/runtime/request_lifecycle.cpp:200-218).
 This module holds no device memory; :mod:`celeg_b200.cache.storage` does.
@@ -241,6 +245,34 @@ class CacheManager:
         self._live[request_id] = cache
         return cache
 
+    def fork(self, request_id: Hashable, new_id: Hashable) -> Tuple[RequestCache, List[List[Tuple[int, int, int]]]]:
+        """A new request that stands where ``request_id`` stands: it shares its full pages and gets a page of its own for
+        a last one that is partly filled, all or nothing. Returns its holdings and, per group, the copies that the
+        caller has to make before either of them goes on: (page, new page, positions written in it), and of the
+        state slot."""
+        source = self.get(request_id)
+        full, rest = divmod(source.tokens, self.page_tokens)
+        ends = [table[full] if rest else NO_PAGE for table in source.tables]
+        for group, page in zip(self.groups, ends):
+            if page != NO_PAGE and group.pool.free_pages < 1:
+                raise OutOfPages(f"the fork of request {request_id!r} needs a page of group {group.key}, none is free")
+        cache = self.open(new_id)
+        copies: List[List[Tuple[int, int, int]]] = []
+        for index, (group, page) in enumerate(zip(self.groups, ends)):
+            shared = source.tables[index][:full]
+            group.pool.retain([held for held in shared if held != NO_PAGE])
+            moves = []
+            if rest:
+                taken = group.pool.allocate(1) if page != NO_PAGE else [NO_PAGE]
+                assert taken is not None
+                shared = shared + taken
+                moves = [(page, taken[0], rest)] if page != NO_PAGE else []
+            cache._append(index, shared)
+            cache.first_live_page[index] = min(source.first_live_page[index], len(shared))
+            copies.append(moves)
+        cache.tokens = source.tokens
+        return cache, copies
+
     def reserve(self, cache: RequestCache, new_total: int) -> None:
         """Make room for positions up to ``new_total`` in every group, all or nothing."""
         if cache.closed:
@@ -301,18 +333,23 @@ class CacheManager:
 
     # ----------------------------------------------------------------- checking
     def check_invariants(self) -> None:
-        """No page lost, none held twice, none both free and held; the same for slots."""
+        """No page lost, none both free and held, each held as often as it is referred to (once, unless requests were
+        forked), only full pages by several; the same for slots."""
         for index, group in enumerate(self.groups):
-            held: Dict[int, Hashable] = {}
+            held: Dict[int, List[Hashable]] = {}
             for cache in self._live.values():
-                for page in cache.held_pages(index):
-                    if page in held:
-                        raise PageError(f"page {page} of group {group.key} is held by {held[page]!r} "
-                                        f"and {cache.request_id!r}")
-                    held[page] = cache.request_id
-                    if group.pool.ref_count(page) != 1:
-                        raise PageError(f"page {page} of group {group.key} is held with ref count "
-                                        f"{group.pool.ref_count(page)}")
+                full = cache.tokens // self.page_tokens
+                for logical, page in enumerate(cache.tables[index]):
+                    if page == NO_PAGE:
+                        continue
+                    held.setdefault(page, []).append((cache.request_id, logical < full))
+            for page, holders in held.items():
+                if group.pool.ref_count(page) != len(holders):
+                    raise PageError(f"page {page} of group {group.key} is held by {[name for name, _ in holders]!r} "
+                                    f"with ref count {group.pool.ref_count(page)}")
+                if len(holders) > 1 and not all(full for _, full in holders):
+                    raise PageError(f"page {page} of group {group.key} is held by {[name for name, _ in holders]!r} "
+                                    f"and not full")
             if len(held) != group.pool.used_pages:
                 raise PageError(f"group {group.key}: {group.pool.used_pages} pages are out of the pool, "
                                 f"requests hold {len(held)}")

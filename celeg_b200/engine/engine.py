@@ -1,15 +1,20 @@
 """The Python entry point: an engine over one model folder, with celeg's engine calls
 (``ConcurrentEngine``: include/celeg/backend/cuda/concurrency.hpp:36-70; C API
 include/celeg/api.h:142-179): submit, step, poll, status, cancel, release, metrics; plus
-``generate`` for the common case and ``forward`` for the raw step."""
+``generate`` for the common case, ``forward`` for the raw step, ``fork`` for a second request that goes on where
+one stands, ``score`` for the log probabilities of given tokens."""
 from __future__ import annotations
 
+import math
 import threading
 import time
+from dataclasses import dataclass
 from typing import Dict, Iterable, List, Optional, Sequence, Tuple, Union
 
+import numpy as np
 import torch
 
+from .. import kernels
 from ..parts.options import KernelOptions
 from ..sampling import Sampler, SamplingParams
 from .loading import LoadedModel, load_model
@@ -94,6 +99,22 @@ class _Runner:
         metrics.gpu_seconds += self._gpu_seconds
         self._sample_seconds = 0.0
         self._gpu_seconds = 0.0
+
+
+SCORED_TOKENS = 512          # positions of a prompt whose logits are held at a time (128 MB at a vocabulary of 65,536)
+
+
+@dataclass
+class TokenScores:
+    """Entry i belongs to the prompt's token i + 1, given the tokens before it."""
+    logprobs: List[float]
+    entropy: List[float]
+    top: List[List[Tuple[int, float]]]      # (token, log probability), most likely first
+
+    @property
+    def total(self) -> float:
+        """The log probability of the whole prompt behind its first token."""
+        return math.fsum(self.logprobs)
 
 
 class Engine:
@@ -222,6 +243,58 @@ class Engine:
     def end(self, request_id) -> None:
         with self._lock:
             self.loaded.step.end(request_id)
+
+    def fork(self, request_id, new_id) -> None:
+        """``new_id`` becomes a request of :meth:`forward` that stands where ``request_id`` stands: what that has been fed
+        need not be fed again. Cached positions are shared page by page; what both go on with is their own. Either is
+        ended with :meth:`end`."""
+        with torch.cuda.device(self.device), self._lock:
+            source = self.loaded.manager.get(request_id)
+            cache = self.loaded.step.fork(request_id, new_id)
+            self.sampler.seen[cache.slot].copy_(self.sampler.seen[source.slot])
+
+    def score(self, prompts: Union[Sequence[int], Sequence[Sequence[int]]], top: int = 0):
+        """How likely the model finds given tokens: for every prompt a :class:`TokenScores` with the log probability of each
+        token behind the first, given those before it, the entropy of the distribution it was taken from and, with
+        ``top`` (at most 128), the most likely tokens there. One prompt gives one, several give a list. Needs a free
+        state slot and pages for one prompt at a time; unscaled logits (temperature 1, no penalties)."""
+        single = len(prompts) > 0 and not isinstance(prompts[0], (list, tuple, np.ndarray, torch.Tensor))
+        batch = [prompts] if single else list(prompts)
+        vocab = self.loaded.model.vocab_size
+        if not 0 <= top <= min(kernels.MAX_TOP_LOGPROBS, vocab):
+            raise ValueError(f"top must lie in 0..{min(kernels.MAX_TOP_LOGPROBS, vocab)}, got {top}")
+        batch = [[int(token) for token in prompt] for prompt in batch]
+        for prompt in batch:
+            if not prompt:
+                raise ValueError("a prompt to score holds no tokens")
+            if min(prompt) < 0 or max(prompt) >= vocab:
+                raise ValueError(f"token id {min(prompt) if min(prompt) < 0 else max(prompt)} is outside the vocabulary of {vocab}")
+        out = [self._score(prompt, top) for prompt in batch]
+        return out[0] if single else out
+
+    def _score(self, prompt: List[int], top: int) -> "TokenScores":
+        step, device = self.loaded.step, self.device
+        portion = min(step.max_tokens, SCORED_TOKENS)
+        request_id = ("score", object())
+        with torch.cuda.device(device), self._lock:
+            count = len(prompt)
+            follows = torch.tensor(prompt[1:] + [0], dtype=torch.int32, device=device)
+            logprobs, entropy = (torch.empty(count, dtype=torch.float32, device=device) for _ in range(2))
+            top_logprobs = torch.empty((count, top), dtype=torch.float32, device=device)
+            top_tokens = torch.empty((count, top), dtype=torch.int32, device=device)
+            try:
+                for begin in range(0, count - 1, portion):
+                    tokens = prompt[begin:min(begin + portion, count - 1)]
+                    rows, part = len(tokens), slice(begin, begin + len(tokens))
+                    logits = step.run([StepEntry(request_id, tokens, tuple(range(rows)))], auto_begin=True)
+                    kernels.token_logprobs(logits, rows, follows[part], logprobs[part], entropy[part], top_logprobs[part],
+                                           top_tokens[part])
+                step.raise_on_device_error()
+            finally:
+                if self.loaded.manager.find(request_id) is not None:
+                    step.end(request_id)
+            best = [list(zip(ids, values)) for ids, values in zip(top_tokens[:count - 1].tolist(), top_logprobs[:count - 1].tolist())]
+            return TokenScores(logprobs[:count - 1].tolist(), entropy[:count - 1].tolist(), best)
 
 
 def _request_options(options: Optional[RequestOptions], overrides: dict) -> RequestOptions:

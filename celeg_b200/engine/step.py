@@ -125,6 +125,21 @@ class StepFunction:
     def end(self, request_id: Hashable) -> None:
         self.manager.close(request_id)
 
+    def fork(self, request_id: Hashable, new_id: Hashable):
+        """``new_id`` begins where ``request_id`` stands (see CacheManager.fork): full pages are shared, a partly filled
+        last page and the state slot are copied, on the current stream like the steps of both."""
+        source = self.manager.get(request_id)
+        cache, copies = self.manager.fork(request_id, new_id)
+        try:
+            for k, v, moves in zip(self.storage.k, self.storage.v, copies):
+                if moves:
+                    kernels.copy_pages(k, v, moves)
+            self.storage.state[cache.slot].copy_(self.storage.state[source.slot])
+        except Exception:
+            self.manager.close(new_id)
+            raise
+        return cache
+
     def position_of(self, request_id: Hashable) -> int:
         return self.manager.get(request_id).tokens
 
