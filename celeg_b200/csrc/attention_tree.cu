@@ -4,8 +4,12 @@
 // The general kernel takes float32 and bfloat16, any head size up to 256 and any page size. Everything is float32: a block has
 // 32 rows (node, query head of a group) of one kv head and walks its keys 64 at a time. 128 threads: for the scores a thread
 // has 4 rows x 4 keys, for the weighted sum 4 rows x 4 columns of every 64, operands from shared memory four numbers at a time.
+// Keys and values come as they are stored, by asynchronous copies where rows are whole 16-byte pieces, the next tile under
+// this one's products where two fit.
 #include "attention_tree.cuh"
 #include "attention_tree_tcgen05.h"
+
+#include <type_traits>
 
 namespace celeg_b200 {
 
@@ -13,16 +17,18 @@ constexpr int kSimtThreads = 128;
 constexpr int kSimtRows = 32;
 constexpr int kSimtKeys = 64;
 
-__host__ __device__ inline int simt_pitch(int head_dim) {
-    // rows of 16-byte pieces, eight consecutive rows in different banks
-    const int four = (head_dim + 3) / 4 * 4;
-    return four % 32 == 0 ? four + 4 : four;
-}
-
-inline size_t simt_smem(int head_dim, int columns) {
-    const size_t q_k = (size_t)(kSimtRows + kSimtKeys) * simt_pitch(head_dim);
-    return (q_k + (size_t)kSimtKeys * columns + kSimtRows * (kSimtKeys + 4)) * sizeof(float) + kSimtKeys * (sizeof(int) + sizeof(long long));
-}
+// Shared memory of a block, in the order of the members. Rows of keys are 16-byte pieces, neighbours in different banks.
+template <typename A, int COLUMNS>
+struct SimtLayout {
+    static constexpr int kWidth = 64 * COLUMNS;                           // a row's numbers, padded
+    static constexpr int kPitch = kWidth + 16 / (int)sizeof(A);
+    static constexpr int kQPitch = kWidth + 4, kWeightPitch = kSimtKeys + 4;
+    static constexpr int kStages = COLUMNS == 4 && sizeof(A) == 4 ? 1 : 2;
+    static constexpr size_t kStageBytes = (size_t)kSimtKeys * (kPitch + kWidth) * sizeof(A);
+    static constexpr size_t kQAt = kStages * kStageBytes, kWeightsAt = kQAt + (size_t)kSimtRows * kQPitch * 4;
+    static constexpr size_t kOffsetsAt = kWeightsAt + (size_t)kSimtRows * kWeightPitch * 4, kPositionsAt = kOffsetsAt + 3 * kSimtKeys * 8;
+    static constexpr size_t kBytes = kPositionsAt + 3 * kSimtKeys * 4;
+};
 
 template <typename A>
 __device__ __forceinline__ float4 load_four(const A* p);
@@ -36,57 +42,53 @@ __device__ __forceinline__ float4 load_four<__nv_bfloat16>(const __nv_bfloat16* 
     return make_float4(lo.x, lo.y, hi.x, hi.y);
 }
 
-// A row of `head_dim` numbers in global memory, four of them from column c on (zeros past the end).
-template <typename A, bool FOUR>
-__device__ __forceinline__ float4 row_four(const A* row, int c, int head_dim) {
-    if (FOUR) return load_four<A>(row + c);
-    float4 v;
-    v.x = c < head_dim ? to_float(row[c]) : 0.0f;
-    v.y = c + 1 < head_dim ? to_float(row[c + 1]) : 0.0f;
-    v.z = c + 2 < head_dim ? to_float(row[c + 2]) : 0.0f;
-    v.w = c + 3 < head_dim ? to_float(row[c + 3]) : 0.0f;
-    return v;
-}
-
-// COLUMNS: columns of the output in units of 64 (head_dim <= 64 * COLUMNS). FOUR: rows are read four numbers at a time.
-template <typename A, int COLUMNS, bool FOUR>
+// COLUMNS: columns of the output in units of 64 (head_dim <= 64 * COLUMNS). PIECES: rows are whole 16-byte pieces on 16-byte
+// addresses.
+template <typename A, int COLUMNS, bool PIECES>
 __global__ void __launch_bounds__(kSimtThreads) attention_tree_simt_kernel(const TreeParams p) {
-    extern __shared__ __align__(16) float smem[];
-    const int d = p.head_dim, pitch = simt_pitch(d);
-    float* q_s = smem;                                      // [rows][pitch]
-    float* k_s = q_s + kSimtRows * pitch;                   // [keys][pitch]
-    float* v_s = k_s + kSimtKeys * pitch;                   // [keys][64 * COLUMNS]
-    float* w_s = v_s + kSimtKeys * 64 * COLUMNS;            // [rows][keys + 4]
-    long long* offset_s = reinterpret_cast<long long*>(w_s + kSimtRows * (kSimtKeys + 4));      // [keys], -1: no such key
-    int* position_s = reinterpret_cast<int*>(offset_s + kSimtKeys);                             // [keys]
+    extern __shared__ __align__(16) unsigned char simt_smem[];
+    using L = SimtLayout<A, COLUMNS>;
+    float* q_s = reinterpret_cast<float*>(simt_smem + L::kQAt);                          // [rows][kQPitch]
+    float* w_s = reinterpret_cast<float*>(simt_smem + L::kWeightsAt);                    // [rows][kWeightPitch]
+    long long* offset_s = reinterpret_cast<long long*>(simt_smem + L::kOffsetsAt);       // [3][keys], -1: no such key
+    int* position_s = reinterpret_cast<int*>(simt_smem + L::kPositionsAt);               // [3][keys]
     __shared__ int lowest_s;
 
-    const int tid = threadIdx.x, kx = tid & 15, ry = tid >> 4;
+    const int tid = threadIdx.x, kx = tid & 15, ry = tid >> 4, d = p.head_dim;
     const int span = blockIdx.z, split = blockIdx.x;
     const int tiles = (p.max_nodes * p.group + kSimtRows - 1) / kSimtRows;
     const int kvh = blockIdx.y / tiles, row0 = (blockIdx.y % tiles) * kSimtRows;
+    chain_release();
+    chain_wait();
     const TreeSpan s = tree_span(p, span);
     const int rows = s.nodes * p.group;
     if (row0 >= rows) return;
     const int* table = p.block_table + (size_t)span * p.table_stride;
     const A* q = static_cast<const A*>(p.q);
+    const A* k = static_cast<const A*>(p.k_cache);
+    const A* v = static_cast<const A*>(p.v_cache);
 
     // the keys of this block: from the first that any of its rows sees, in `splits` pieces of whole tiles
     if (tid == 0) lowest_s = 0x7fffffff;
     __syncthreads();
     if (p.window && tid < kSimtRows && row0 + tid < rows) atomicMin(&lowest_s, p.positions[s.begin + (row0 + tid) / p.group]);
-    for (int i = tid; i < kSimtRows * (pitch / 4); i += kSimtThreads) {
-        const int r = i / (pitch / 4), c = (i % (pitch / 4)) * 4, row = row0 + r;
-        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (row < rows && c < d)
-            v = row_four<A, FOUR>(q + (size_t)(s.begin + row / p.group) * p.q_row_stride + (size_t)(kvh * p.group + row % p.group) * d, c, d);
-        *reinterpret_cast<float4*>(q_s + r * pitch + c) = v;
+    for (int i = tid; i < kSimtRows * L::kWidth; i += kSimtThreads) {
+        const int r = i / L::kWidth, c = i % L::kWidth, row = row0 + r;
+        q_s[r * L::kQPitch + c] = row < rows && c < d
+            ? to_float(q[(size_t)(s.begin + row / p.group) * p.q_row_stride + (size_t)(kvh * p.group + row % p.group) * d + c]) : 0.0f;
+    }
+    if (d % 4 != 0) {       // (what a row's last four numbers reach past its end: zeros, for good)
+        for (int i = tid; i < L::kStages * kSimtKeys; i += kSimtThreads) {
+            A* stage = reinterpret_cast<A*>(simt_smem + (i / kSimtKeys) * L::kStageBytes);
+            for (int c = d; c < (d + 3) / 4 * 4; ++c) stage[(i % kSimtKeys) * L::kPitch + c] = from_float<A>(0.0f);
+        }
     }
     __syncthreads();
     const int first = p.window ? tree_first_place(p, s, lowest_s) : 0, last = s.context + s.nodes;
     const int per_split = ((last - first + p.splits - 1) / p.splits + kSimtKeys - 1) / kSimtKeys * kSimtKeys;
     const long long from = (long long)first + (long long)split * per_split;
     const int end = (int)min((long long)last, from + per_split);
+    const int key_first = (int)min(from, (long long)last), count = end > key_first ? (end - key_first + kSimtKeys - 1) / kSimtKeys : 0;
 
     int node_position[4];
     const unsigned* mask[4];
@@ -104,48 +106,84 @@ __global__ void __launch_bounds__(kSimtThreads) attention_tree_simt_kernel(const
             for (int e = 0; e < 4; ++e) acc[i][j][e] = 0.0f;
     }
 
-    for (long long base = from; base < end; base += kSimtKeys) {
-        const int key0 = (int)base, count = min(kSimtKeys, end - key0);
-        if (tid < kSimtKeys) {
-            const int place = key0 + tid;
-            long long offset = -1;
-            int position = place;
-            if (tid < count) {
-                const int page = tree_page(p, table, place);
-                if (page >= 0) offset = (long long)page * p.page_stride + ((long long)kvh * p.page_tokens + place % p.page_tokens) * d;
-                if (p.window && place >= s.context) position = p.positions[s.begin + place - s.context];
+    // where the keys of tile n lie, and their positions
+    auto look_up = [&](int n) {
+        if (tid >= kSimtKeys || n >= count) return;
+        const int place = key_first + n * kSimtKeys + tid;
+        long long offset = -1;
+        int position = place;
+        if (place < end) {
+            const int page = tree_page(p, table, place);
+            if (page >= 0) offset = (long long)page * p.page_stride + ((long long)kvh * p.page_tokens + place % p.page_tokens) * d;
+            if (p.window && place >= s.context) position = p.positions[s.begin + place - s.context];
+        }
+        offset_s[n % 3 * kSimtKeys + tid] = offset;
+        position_s[n % 3 * kSimtKeys + tid] = position;
+    };
+    auto bring = [&](int n) {
+        unsigned char* stage = simt_smem + (n % L::kStages) * L::kStageBytes;
+        A* k_s = reinterpret_cast<A*>(stage);
+        A* v_s = k_s + kSimtKeys * L::kPitch;
+        if (PIECES) {
+            constexpr int kPiece = 16 / (int)sizeof(A), kPerRow = L::kWidth / kPiece, kRowsATurn = kSimtThreads / kPerRow;
+            const int c = tid % kPerRow * kPiece, r0 = tid / kPerRow;
+#pragma unroll 8
+            for (int u = 0; u < kSimtKeys / kRowsATurn; ++u) {
+                const int r = r0 + u * kRowsATurn;
+                const long long offset = offset_s[n % 3 * kSimtKeys + r];
+                const bool there = offset >= 0 && c < d;
+                const long long at = there ? offset + c : 0;
+                const unsigned bytes = there ? 16 : 0;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"((unsigned)__cvta_generic_to_shared(k_s + r * L::kPitch + c)), "l"(k + at), "r"(bytes) : "memory");
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"((unsigned)__cvta_generic_to_shared(v_s + r * L::kWidth + c)), "l"(v + at), "r"(bytes) : "memory");
             }
-            offset_s[tid] = offset;
-            position_s[tid] = position;
+        } else {
+            for (int i = tid; i < kSimtKeys * L::kWidth; i += kSimtThreads) {
+                const int r = i / L::kWidth, c = i % L::kWidth;
+                if (c >= d) continue;
+                const long long offset = offset_s[n % 3 * kSimtKeys + r];
+                k_s[r * L::kPitch + c] = offset >= 0 ? k[offset + c] : from_float<A>(0.0f);
+                v_s[r * L::kWidth + c] = offset >= 0 ? v[offset + c] : from_float<A>(0.0f);
+            }
         }
-        __syncthreads();
-        const A* k = static_cast<const A*>(p.k_cache);
-        const A* v = static_cast<const A*>(p.v_cache);
-        for (int i = tid; i < kSimtKeys * (pitch / 4); i += kSimtThreads) {
-            const int r = i / (pitch / 4), c = (i % (pitch / 4)) * 4;
-            const long long offset = offset_s[r];
-            *reinterpret_cast<float4*>(k_s + r * pitch + c) =
-                offset >= 0 && c < d ? row_four<A, FOUR>(k + offset, c, d) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        asm volatile("cp.async.commit_group;\n" ::: "memory");
+    };
+
+    look_up(0);
+    look_up(1);
+    __syncthreads();
+    if (L::kStages > 1 && count > 0) bring(0);
+    for (int n = 0; n < count; ++n) {
+        if (L::kStages > 1) {
+            if (n + 1 < count) bring(n + 1);
+            look_up(n + 2);
+            if (n + 1 < count) asm volatile("cp.async.wait_group 1;\n" ::: "memory");
+            else asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+        } else {
+            bring(n);
+            look_up(n + 2);
+            asm volatile("cp.async.wait_group 0;\n" ::: "memory");
         }
-        for (int i = tid; i < kSimtKeys * 16 * COLUMNS; i += kSimtThreads) {
-            const int r = i / (16 * COLUMNS), c = (i % (16 * COLUMNS)) * 4;
-            const long long offset = offset_s[r];
-            *reinterpret_cast<float4*>(v_s + r * 64 * COLUMNS + c) =
-                offset >= 0 && c < d ? row_four<A, FOUR>(v + offset, c, d) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        }
-        __syncthreads();
+        const int key0 = key_first + n * kSimtKeys, held = min(kSimtKeys, end - key0);
+        const long long* offsets = offset_s + n % 3 * kSimtKeys;
+        const int* key_positions = position_s + n % 3 * kSimtKeys;
+        const A* k_s = reinterpret_cast<const A*>(simt_smem + (n % L::kStages) * L::kStageBytes);
+        const A* v_s = k_s + kSimtKeys * L::kPitch;
+        // every row sees every key of the tile, unless the tile reaches into the tree, the window's edge or a missing page
+        const bool whole = __syncthreads_and(p.window == 0 && key0 + kSimtKeys <= s.context && (tid >= kSimtKeys || offsets[tid] >= 0));
 
         float score[4][4];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) score[i][j] = 0.0f;
+#pragma unroll 4
         for (int c = 0; c < d; c += 4) {
             float4 a[4], b[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const float4*>(q_s + (ry * 4 + i) * pitch + c);
+            for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const float4*>(q_s + (ry * 4 + i) * L::kQPitch + c);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const float4*>(k_s + (kx + 16 * j) * pitch + c);
+            for (int j = 0; j < 4; ++j) b[j] = load_four<A>(k_s + (kx + 16 * j) * L::kPitch + c);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -156,8 +194,6 @@ __global__ void __launch_bounds__(kSimtThreads) attention_tree_simt_kernel(const
                     score[i][j] = fmaf(a[i].w, b[j].w, score[i][j]);
                 }
         }
-        // every row sees every key of the tile, unless the tile reaches into the tree, the window's edge or a missing page
-        const bool whole = __syncthreads_and(p.window == 0 && key0 + kSimtKeys <= s.context && (tid >= kSimtKeys || offset_s[tid] >= 0));
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             float top = -INFINITY;
@@ -166,7 +202,7 @@ __global__ void __launch_bounds__(kSimtThreads) attention_tree_simt_kernel(const
                 float x = score[i][j];
                 x = p.cap_out > 0.0f ? p.cap_out * tanhf(x * p.cap_in) : x * p.scale;
                 const int at = kx + 16 * j;
-                if (!whole && (offset_s[at] < 0 || !tree_sees(p, s, mask[i], node_position[i], key0 + at, position_s[at]))) x = -INFINITY;
+                if (!whole && (offsets[at] < 0 || !tree_sees(p, s, mask[i], node_position[i], key0 + at, key_positions[at]))) x = -INFINITY;
                 score[i][j] = x;
                 top = fmaxf(top, x);
             }
@@ -180,7 +216,7 @@ __global__ void __launch_bounds__(kSimtThreads) attention_tree_simt_kernel(const
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const float w = expf(score[i][j] - base_max);
-                w_s[(ry * 4 + i) * (kSimtKeys + 4) + kx + 16 * j] = w;
+                w_s[(ry * 4 + i) * L::kWeightPitch + kx + 16 * j] = w;
                 sum += w;
             }
             run_sum[i] = run_sum[i] * factor + sum;                      // (this lane's share of the row)
@@ -190,30 +226,34 @@ __global__ void __launch_bounds__(kSimtThreads) attention_tree_simt_kernel(const
                 for (int e = 0; e < 4; ++e) acc[i][j][e] *= factor;
         }
         __syncwarp();                        // (a warp's 8 rows of weights are read by this warp alone)
-        for (int n = 0; n < count; n += 4) {
-            float w[4][4];
+        // `masked`: a weight of 0 is a key that the row does not see, whose value, whatever it is, must not reach it
+        auto add_up = [&](auto masked) {
+#pragma unroll 2
+            for (int t = 0; t < held; t += 4) {
+                float w[4][4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float4 four = *reinterpret_cast<const float4*>(w_s + (ry * 4 + i) * (kSimtKeys + 4) + n);
-                w[i][0] = four.x, w[i][1] = four.y, w[i][2] = four.z, w[i][3] = four.w;
-            }
+                for (int i = 0; i < 4; ++i) {
+                    const float4 four = *reinterpret_cast<const float4*>(w_s + (ry * 4 + i) * L::kWeightPitch + t);
+                    w[i][0] = four.x, w[i][1] = four.y, w[i][2] = four.z, w[i][3] = four.w;
+                }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
+                for (int e = 0; e < 4; ++e) {
 #pragma unroll
-                for (int j = 0; j < COLUMNS; ++j) {
-                    const float4 x = *reinterpret_cast<const float4*>(v_s + (n + e) * 64 * COLUMNS + j * 64 + kx * 4);
+                    for (int j = 0; j < COLUMNS; ++j) {
+                        const float4 x = load_four<A>(v_s + (t + e) * L::kWidth + j * 64 + kx * 4);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        // (a masked key's weight is 0: its value, whatever it is, must not reach the row)
-                        if (!whole && w[i][e] == 0.0f) continue;
-                        acc[i][j][0] = fmaf(w[i][e], x.x, acc[i][j][0]);
-                        acc[i][j][1] = fmaf(w[i][e], x.y, acc[i][j][1]);
-                        acc[i][j][2] = fmaf(w[i][e], x.z, acc[i][j][2]);
-                        acc[i][j][3] = fmaf(w[i][e], x.w, acc[i][j][3]);
+                        for (int i = 0; i < 4; ++i) {
+                            if (decltype(masked)::value && w[i][e] == 0.0f) continue;
+                            acc[i][j][0] = fmaf(w[i][e], x.x, acc[i][j][0]);
+                            acc[i][j][1] = fmaf(w[i][e], x.y, acc[i][j][1]);
+                            acc[i][j][2] = fmaf(w[i][e], x.z, acc[i][j][2]);
+                            acc[i][j][3] = fmaf(w[i][e], x.w, acc[i][j][3]);
+                        }
                     }
                 }
             }
-        }
+        };
+        if (whole) add_up(std::false_type()); else add_up(std::true_type());
         __syncthreads();
     }
 
@@ -260,39 +300,51 @@ __global__ void __launch_bounds__(256) attention_tree_join_kernel(const TreePara
     const int lane = threadIdx.x & 31, d = p.head_dim;
     const long long token = unit / p.q_heads;
     if (token < p.span_begin[0] || token >= min(p.span_begin[p.spans], p.tokens)) return;       // (rows of no span)
-    const float* ml = p.part_ml + unit * p.splits * 2;
-    float top = -INFINITY;
-    for (int i = lane; i < p.splits; i += 32) top = fmaxf(top, ml[2 * i]);
-    top = warp_max(top);
-    float total = 0.0f;
-    for (int i = lane; i < p.splits; i += 32) total += ml[2 * i] == -INFINITY ? 0.0f : ml[2 * i + 1] * exp2f(ml[2 * i] - top);
-    total = warp_sum(total);
+    // a lane has the factors of two pieces (64 at most); the outputs of four pieces are asked for together
+    const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + unit * p.splits;
+    const float2 none = make_float2(-INFINITY, 0.0f);
+    const float2 low = lane < p.splits ? ml[lane] : none, high = lane + 32 < p.splits ? ml[lane + 32] : none;
+    const float top = warp_max(fmaxf(low.x, high.x));
+    const float low_factor = low.x == -INFINITY ? 0.0f : exp2f(low.x - top), high_factor = high.x == -INFINITY ? 0.0f : exp2f(high.x - top);
+    float total = warp_sum(low.y * low_factor + high.y * high_factor);
     if (p.sinks && top != -INFINITY) total += exp2f(p.sinks[unit % p.q_heads] * 1.4426950408889634f - top);
     const float inv = top == -INFINITY ? 0.0f : 1.0f / total;
-    for (int c = lane; c < d; c += 32) {
+    for (int c = lane; c < d + lane; c += 32) {        // (every lane comes to every exchange)
         float sum = 0.0f;
-        for (int i = 0; i < p.splits; ++i) {
-            const float m = ml[2 * i];
-            if (m != -INFINITY) sum = fmaf(p.part_o[(unit * p.splits + i) * d + c], exp2f(m - top), sum);
+        for (int i0 = 0; i0 < p.splits; i0 += 4) {
+            float factor[4], x[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int i = i0 + u;
+                factor[u] = __shfl_sync(0xffffffffu, i < 32 ? low_factor : high_factor, i & 31);
+                x[u] = i < p.splits && c < d && factor[u] != 0.0f ? p.part_o[(unit * p.splits + i) * d + c] : 0.0f;
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) sum = i0 + u < p.splits ? fmaf(x[u], factor[u], sum) : sum;
         }
-        static_cast<A*>(p.out)[unit * d + c] = from_float<A>(sum * inv);
+        if (c < d) static_cast<A*>(p.out)[unit * d + c] = from_float<A>(sum * inv);
     }
 }
 
-template <typename A, bool FOUR>
-static int launch_simt(const TreeParams& p, cudaStream_t stream) {
-    auto kernel = attention_tree_simt_kernel<A, 4, FOUR>;
-    int columns = 4;
-    if (p.head_dim <= 64) kernel = attention_tree_simt_kernel<A, 1, FOUR>, columns = 1;
-    else if (p.head_dim <= 128) kernel = attention_tree_simt_kernel<A, 2, FOUR>, columns = 2;
-    const size_t smem = simt_smem(p.head_dim, 64 * columns);
+template <typename A, int COLUMNS, bool PIECES>
+static int launch_simt_columns(const TreeParams& p, cudaStream_t stream) {
+    auto kernel = attention_tree_simt_kernel<A, COLUMNS, PIECES>;
+    constexpr size_t smem = SimtLayout<A, COLUMNS>::kBytes;
+    static_assert(smem <= 227 * 1024, "a block's shared memory");
     if (smem > 40 * 1024) {
         const cudaError_t status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         CELEG_REQUIRE(status == cudaSuccess, "attention_tree: %s", cudaGetErrorString(status));
     }
     const int tiles = (p.max_nodes * p.group + kSimtRows - 1) / kSimtRows;
-    kernel<<<dim3(p.splits, p.kv_heads * tiles, p.spans), kSimtThreads, smem, stream>>>(p);
+    launch_chained(kernel, dim3(p.splits, p.kv_heads * tiles, p.spans), dim3(kSimtThreads), smem, stream, p);
     return check_launch("attention_tree");
+}
+
+template <typename A, bool PIECES>
+static int launch_simt(const TreeParams& p, cudaStream_t stream) {
+    if (p.head_dim <= 64) return launch_simt_columns<A, 1, PIECES>(p, stream);
+    if (p.head_dim <= 128) return launch_simt_columns<A, 2, PIECES>(p, stream);
+    return launch_simt_columns<A, 4, PIECES>(p, stream);
 }
 
 template <typename A>
@@ -392,15 +444,14 @@ CELEG_API int celeg_attention_tree(const void* q, long long q_row_stride, void* 
     if (p.splits <= tile.cluster) p.part_o = nullptr;
     p.part_ml = p.part_o ? scratch + units * p.splits * head_dim : nullptr;
     const size_t size = act_dtype == kFloat32 ? 4 : 2;
-    const bool four = head_dim % 4 == 0 && page_stride % 4 == 0 && q_row_stride % 4 == 0 &&
-                      (((size_t)q | (size_t)k_cache | (size_t)v_cache) & (4 * size - 1)) == 0;
+    const bool pieces = head_dim * size % 16 == 0 && page_stride * size % 16 == 0 && (((size_t)k_cache | (size_t)v_cache) & 15) == 0;
     int code;
     if (tensor_cores)
         code = launch_tree_tcgen05(p, stream);
     else if (act_dtype == kFloat32)
-        code = four ? launch_simt<float, true>(p, stream) : launch_simt<float, false>(p, stream);
+        code = pieces ? launch_simt<float, true>(p, stream) : launch_simt<float, false>(p, stream);
     else
-        code = four ? launch_simt<__nv_bfloat16, true>(p, stream) : launch_simt<__nv_bfloat16, false>(p, stream);
+        code = pieces ? launch_simt<__nv_bfloat16, true>(p, stream) : launch_simt<__nv_bfloat16, false>(p, stream);
     if (code != 0 || !p.part_o) return code;
     return act_dtype == kFloat32 ? launch_join<float>(p, stream) : launch_join<__nv_bfloat16>(p, stream);
 }
