@@ -3,11 +3,16 @@
 //
 // The general kernel takes float32 and bfloat16, any head size up to 256 and any page size. Everything is float32: a block has
 // 32 rows (node, query head of a group) of one kv head and walks its keys 64 at a time. 128 threads: for the scores a thread
-// has 4 rows x 4 keys, for the weighted sum 4 rows x 4 columns of every 64, operands from shared memory four numbers at a time.
-// Keys and values come as they are stored, by asynchronous copies where rows are whole 16-byte pieces, the next tile under
-// this one's products where two fit.
+// has 4 rows x 4 keys, for the weighted sum 4 rows x 4 columns of every 64, operands from shared memory four numbers at a
+// time, products packed two an instruction (neighbouring numbers of a score's sum, neighbouring columns of an output). (With 8
+// rows a thread an operand serves twice as many products, but a step's instructions, which come once a step, no longer
+// arrive as fast as they run: two requests of 24 nodes x 1,500 positions in float32 took 51 us, 36 with 4.)
+// Keys and values come as they are stored, by asynchronous copies where rows are whole 16-byte pieces: of bfloat16 the next tile
+// under this one's products, of float32 one tile at a time, which leaves room for twice as many blocks an SM (eight requests of
+// 32 nodes x 4,096 positions: 256 us, 378 with two tiles).
 #include "attention_tree.cuh"
 #include "attention_tree_tcgen05.h"
+#include "tcgen05.cuh"
 
 #include <type_traits>
 
@@ -23,7 +28,7 @@ struct SimtLayout {
     static constexpr int kWidth = 64 * COLUMNS;                           // a row's numbers, padded
     static constexpr int kPitch = kWidth + 16 / (int)sizeof(A);
     static constexpr int kQPitch = kWidth + 4, kWeightPitch = kSimtKeys + 4;
-    static constexpr int kStages = COLUMNS == 4 && sizeof(A) == 4 ? 1 : 2;
+    static constexpr int kStages = sizeof(A) == 4 ? 1 : 2;
     static constexpr size_t kStageBytes = (size_t)kSimtKeys * (kPitch + kWidth) * sizeof(A);
     static constexpr size_t kQAt = kStages * kStageBytes, kWeightsAt = kQAt + (size_t)kSimtRows * kQPitch * 4;
     static constexpr size_t kOffsetsAt = kWeightsAt + (size_t)kSimtRows * kWeightPitch * 4, kPositionsAt = kOffsetsAt + 3 * kSimtKeys * 8;
@@ -48,6 +53,7 @@ template <typename A, int COLUMNS, bool PIECES>
 __global__ void __launch_bounds__(kSimtThreads) attention_tree_simt_kernel(const TreeParams p) {
     extern __shared__ __align__(16) unsigned char simt_smem[];
     using L = SimtLayout<A, COLUMNS>;
+    constexpr int RT = kSimtRows / 8;                                                    // rows a thread
     float* q_s = reinterpret_cast<float*>(simt_smem + L::kQAt);                          // [rows][kQPitch]
     float* w_s = reinterpret_cast<float*>(simt_smem + L::kWeightsAt);                    // [rows][kWeightPitch]
     long long* offset_s = reinterpret_cast<long long*>(simt_smem + L::kOffsetsAt);       // [3][keys], -1: no such key
@@ -90,12 +96,13 @@ __global__ void __launch_bounds__(kSimtThreads) attention_tree_simt_kernel(const
     const int end = (int)min((long long)last, from + per_split);
     const int key_first = (int)min(from, (long long)last), count = end > key_first ? (end - key_first + kSimtKeys - 1) / kSimtKeys : 0;
 
-    int node_position[4];
-    const unsigned* mask[4];
-    float run_max[4], run_sum[4], acc[4][COLUMNS][4];
+    int node_position[RT];
+    const unsigned* mask[RT];
+    float run_max[RT], run_sum[RT];
+    unsigned long long acc[RT][COLUMNS][2];                // columns in pairs
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int node = s.begin + min(row0 + ry * 4 + i, rows - 1) / p.group;
+    for (int i = 0; i < RT; ++i) {
+        const int node = s.begin + min(row0 + ry * RT + i, rows - 1) / p.group;
         node_position[i] = p.window ? p.positions[node] : 0;
         mask[i] = p.ancestors + (size_t)node * p.words;
         run_max[i] = -INFINITY;
@@ -103,7 +110,7 @@ __global__ void __launch_bounds__(kSimtThreads) attention_tree_simt_kernel(const
 #pragma unroll
         for (int j = 0; j < COLUMNS; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[i][j][e] = 0.0f;
+            for (int e = 0; e < 2; ++e) acc[i][j][e] = 0ull;
     }
 
     // where the keys of tile n lie, and their positions
@@ -172,38 +179,40 @@ __global__ void __launch_bounds__(kSimtThreads) attention_tree_simt_kernel(const
         // every row sees every key of the tile, unless the tile reaches into the tree, the window's edge or a missing page
         const bool whole = __syncthreads_and(p.window == 0 && key0 + kSimtKeys <= s.context && (tid >= kSimtKeys || offsets[tid] >= 0));
 
-        float score[4][4];
+        unsigned long long score2[RT][4];                  // the sums over even and odd numbers
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < RT; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) score[i][j] = 0.0f;
-#pragma unroll 4
+            for (int j = 0; j < 4; ++j) score2[i][j] = 0ull;
+#pragma unroll 2
         for (int c = 0; c < d; c += 4) {
-            float4 a[4], b[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const float4*>(q_s + (ry * 4 + i) * L::kQPitch + c);
+            float4 a[RT], b[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) b[j] = load_four<A>(k_s + (kx + 16 * j) * L::kPitch + c);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < RT; ++i) a[i] = *reinterpret_cast<const float4*>(q_s + (ry * RT + i) * L::kQPitch + c);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    score[i][j] = fmaf(a[i].x, b[j].x, score[i][j]);
-                    score[i][j] = fmaf(a[i].y, b[j].y, score[i][j]);
-                    score[i][j] = fmaf(a[i].z, b[j].z, score[i][j]);
-                    score[i][j] = fmaf(a[i].w, b[j].w, score[i][j]);
-                }
+            for (int i = 0; i < RT; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) score2[i][j] = fma_f32x2(pack_f32x2(a[i].x, a[i].y), pack_f32x2(b[j].x, b[j].y), score2[i][j]);
+#pragma unroll
+            for (int i = 0; i < RT; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) score2[i][j] = fma_f32x2(pack_f32x2(a[i].z, a[i].w), pack_f32x2(b[j].z, b[j].w), score2[i][j]);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < RT; ++i) {
+            float score[4];
             float top = -INFINITY;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                float x = score[i][j];
+                float even, odd;
+                unpack_f32x2(score2[i][j], even, odd);
+                float x = even + odd;
                 x = p.cap_out > 0.0f ? p.cap_out * tanhf(x * p.cap_in) : x * p.scale;
                 const int at = kx + 16 * j;
                 if (!whole && (offsets[at] < 0 || !tree_sees(p, s, mask[i], node_position[i], key0 + at, key_positions[at]))) x = -INFINITY;
-                score[i][j] = x;
+                score[j] = x;
                 top = fmaxf(top, x);
             }
 #pragma unroll
@@ -215,39 +224,39 @@ __global__ void __launch_bounds__(kSimtThreads) attention_tree_simt_kernel(const
             float sum = 0.0f;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float w = expf(score[i][j] - base_max);
-                w_s[(ry * 4 + i) * L::kWeightPitch + kx + 16 * j] = w;
+                const float w = expf(score[j] - base_max);
+                w_s[(ry * RT + i) * L::kWeightPitch + kx + 16 * j] = w;
                 sum += w;
             }
             run_sum[i] = run_sum[i] * factor + sum;                      // (this lane's share of the row)
+            const unsigned long long factor2 = pack_f32x2(factor, factor);
 #pragma unroll
             for (int j = 0; j < COLUMNS; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[i][j][e] *= factor;
+                for (int e = 0; e < 2; ++e) acc[i][j][e] = mul_f32x2(acc[i][j][e], factor2);
         }
         __syncwarp();                        // (a warp's 8 rows of weights are read by this warp alone)
         // `masked`: a weight of 0 is a key that the row does not see, whose value, whatever it is, must not reach it
         auto add_up = [&](auto masked) {
 #pragma unroll 2
             for (int t = 0; t < held; t += 4) {
-                float w[4][4];
+                float4 w[RT];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float4 four = *reinterpret_cast<const float4*>(w_s + (ry * 4 + i) * L::kWeightPitch + t);
-                    w[i][0] = four.x, w[i][1] = four.y, w[i][2] = four.z, w[i][3] = four.w;
-                }
+                for (int i = 0; i < RT; ++i) w[i] = *reinterpret_cast<const float4*>(w_s + (ry * RT + i) * L::kWeightPitch + t);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
+                    float4 x[COLUMNS];
 #pragma unroll
-                    for (int j = 0; j < COLUMNS; ++j) {
-                        const float4 x = load_four<A>(v_s + (t + e) * L::kWidth + j * 64 + kx * 4);
+                    for (int j = 0; j < COLUMNS; ++j) x[j] = load_four<A>(v_s + (t + e) * L::kWidth + j * 64 + kx * 4);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            if (decltype(masked)::value && w[i][e] == 0.0f) continue;
-                            acc[i][j][0] = fmaf(w[i][e], x.x, acc[i][j][0]);
-                            acc[i][j][1] = fmaf(w[i][e], x.y, acc[i][j][1]);
-                            acc[i][j][2] = fmaf(w[i][e], x.z, acc[i][j][2]);
-                            acc[i][j][3] = fmaf(w[i][e], x.w, acc[i][j][3]);
+                    for (int i = 0; i < RT; ++i) {
+                        const float weight = e == 0 ? w[i].x : e == 1 ? w[i].y : e == 2 ? w[i].z : w[i].w;
+                        if (decltype(masked)::value && weight == 0.0f) continue;
+                        const unsigned long long both = pack_f32x2(weight, weight);
+#pragma unroll
+                        for (int j = 0; j < COLUMNS; ++j) {
+                            acc[i][j][0] = fma_f32x2(both, pack_f32x2(x[j].x, x[j].y), acc[i][j][0]);
+                            acc[i][j][1] = fma_f32x2(both, pack_f32x2(x[j].z, x[j].w), acc[i][j][1]);
                         }
                     }
                 }
@@ -258,11 +267,11 @@ __global__ void __launch_bounds__(kSimtThreads) attention_tree_simt_kernel(const
     }
 
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < RT; ++i) {
         float sum = run_sum[i];
 #pragma unroll
         for (int lanes = 8; lanes > 0; lanes >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, lanes);
-        const int row = row0 + ry * 4 + i;
+        const int row = row0 + ry * RT + i;
         if (row >= rows) continue;
         const int head = kvh * p.group + row % p.group;
         const size_t unit = (size_t)(s.begin + row / p.group) * p.q_heads + head;
@@ -279,16 +288,20 @@ __global__ void __launch_bounds__(kSimtThreads) attention_tree_simt_kernel(const
             inv = run_max[i] == -INFINITY ? 0.0f : 1.0f / sum;
         }
 #pragma unroll
-        for (int j = 0; j < COLUMNS; ++j)
+        for (int j = 0; j < COLUMNS; ++j) {
+            float o[4];
+            unpack_f32x2(acc[i][j][0], o[0], o[1]);
+            unpack_f32x2(acc[i][j][1], o[2], o[3]);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int c = j * 64 + kx * 4 + e;
                 if (c >= d) continue;
                 if (p.splits > 1)
-                    p.part_o[(unit * p.splits + split) * d + c] = acc[i][j][e];
+                    p.part_o[(unit * p.splits + split) * d + c] = o[e];
                 else
-                    static_cast<A*>(p.out)[unit * d + c] = from_float<A>(acc[i][j][e] * inv);
+                    static_cast<A*>(p.out)[unit * d + c] = from_float<A>(o[e] * inv);
             }
+        }
     }
 }
 
@@ -398,7 +411,7 @@ CELEG_API int celeg_attention_tree(const void* q, long long q_row_stride, void* 
     CELEG_REQUIRE(act_dtype == kFloat32 || act_dtype == kBFloat16, "attention_tree: unknown dtype code %d", act_dtype);
     if (tokens == 0 || spans == 0) return 0;
     const int group = q_heads / kv_heads;
-    const long long tiles = ((long long)max_nodes * group + kSimtRows - 1) / kSimtRows;
+    const long long tiles = ((long long)max_nodes * group + 31) / 32;
     CELEG_REQUIRE(spans <= 65535 && kv_heads * tiles <= 65535 && (long long)max_nodes * group <= 1 << 24,
                   "attention_tree: %d spans of %d nodes on %d heads exceed one launch", spans, max_nodes, q_heads);
     TreeParams p = {};
@@ -436,15 +449,15 @@ CELEG_API int celeg_attention_tree(const void* q, long long q_row_stride, void* 
     const long long units = (long long)tokens * q_heads;
     p.part_o = scratch;
     const bool tensor_cores = act_dtype == kBFloat16 && tree_tcgen05_takes(p);
-    TreeTile tile = {kSimtRows, 296, 4, 1, {0}};
+    const size_t size = act_dtype == kFloat32 ? 4 : 2;
+    const bool pieces = head_dim * size % 16 == 0 && page_stride * size % 16 == 0 && (((size_t)k_cache | (size_t)v_cache) & 15) == 0;
+    TreeTile tile = {kSimtRows, 592, 2, 1, {0}};
     if (tensor_cores) tile = tree_tcgen05_tile(p);
     const long long reach = window > 0 && (long long)window + max_nodes < max_keys ? (long long)window + max_nodes : max_keys;
     p.splits = tree_splits((long long)spans * kv_heads * ((max_nodes * group + tile.rows - 1) / tile.rows), tile, (reach + 63) / 64,
                            scratch ? scratch_elements / (units * (head_dim + 2)) : 0);
     if (p.splits <= tile.cluster) p.part_o = nullptr;
     p.part_ml = p.part_o ? scratch + units * p.splits * head_dim : nullptr;
-    const size_t size = act_dtype == kFloat32 ? 4 : 2;
-    const bool pieces = head_dim * size % 16 == 0 && page_stride * size % 16 == 0 && (((size_t)k_cache | (size_t)v_cache) & 15) == 0;
     int code;
     if (tensor_cores)
         code = launch_tree_tcgen05(p, stream);

@@ -1,12 +1,13 @@
 // Attention of a tree of drafted tokens over the paged cache on the fifth-generation tensor cores: bfloat16, head sizes that are
-// multiples of 8 up to 128, pages of any size (see attention_tree.cuh for the operator).
+// multiples of 8 up to 256, pages of any size (see attention_tree.cuh for the operator).
 //
 //   grid = (row tiles x pieces of the keys, kv heads, spans). A row is a (node, query head of the group) of one kv head, so that
 //   a key is read once for a whole group and tree; keys come in blocks of 64, a piece is a run of whole blocks.
 //   Fourteen warps, one block an SM. Two teams, each of a warp that issues its products (tcgen05.mma: S = Q K^T, and O += P V
 //   with P from tensor memory and V as it lies in the cache) and four warps of softmax, a thread a row. A row tile has 128
 //   rows and the teams take its even and odd blocks of keys, with outputs, maxima and sums of their own; or, where there are
-//   more rows, 256 rows, a team 128 of them, and every block of keys serves both teams. A team's S and P exist twice, so that its
+//   more rows, 256 rows, a team 128 of them, and every block of keys serves both teams. (Above a head size of 128 the outputs of
+//   one team fill the tensor memory: the first team works alone.) A team's S and P exist twice, so that its
 //   products run while its softmax is busy with another block. A step of the softmax is a chain of waits around its
 //   exponentials, which the two teams hide from one another.
 //   Four warps copy K and V: rows of 16-byte pieces by cp.async, written in the layout with the 128-byte swizzle that the
@@ -38,25 +39,26 @@ constexpr int kTtN = 64;                  // keys per block
 constexpr int kTtMaxCluster = 8;          // pieces of the keys that meet in shared memory
 constexpr unsigned kTtTmemColumns = 512;
 
-// D: the head size padded to 64 or 128. Rows of 128 lie in shared memory as two halves of 64 (a swizzled row is 128 bytes).
+// D: the head size padded to 64, 128 or 256. Rows lie in shared memory in parts of 64 numbers (a swizzled row is 128 bytes).
 template <int D, bool PAIRED>
 struct TtLayout {
     static constexpr int kHalves = D / 64;
     static constexpr unsigned kQHalf = kTtM * 128, kKvHalf = kTtN * 128;
     static constexpr unsigned kQBytes = kHalves * kQHalf;       // 16 or 32 KiB a team
     static constexpr unsigned kKvBytes = kHalves * kKvHalf;     // 8 or 16 KiB each for a block's K and V
-    static constexpr int kStages = D == 64 ? 12 : PAIRED ? 5 : 6;
+    static constexpr bool kAlone = D == 256;                    // one team
+    static constexpr int kStages = D == 64 ? 12 : kAlone ? 2 : PAIRED ? 5 : 6;
     static constexpr unsigned kAllQ = PAIRED ? 2 * kQBytes : kQBytes;
-    static constexpr unsigned kSmemBytes = kAllQ + kStages * 2 * kKvBytes + 1024;      // 209 to 225 KiB
+    static constexpr unsigned kSmemBytes = kAllQ + kStages * 2 * kKvBytes + 1024;      // 193 to 225 KiB
     // what meets at the end lies where queries and keys were: rows of results (16-byte pieces of eight rows in different banks),
-    // 2 x 128 and one more of every part, their maxima and sums, the rows' (token, query head) numbers
-    static constexpr int kPitch = D + 4, kMeetRows = 2 * kTtM + 2 * kTtMaxCluster;
+    // 128 a team and one more of every part, their maxima and sums, the rows' (token, query head) numbers
+    static constexpr int kPitch = D + 4, kMeetRows = (kAlone ? 1 : 2) * (kTtM + kTtMaxCluster);
     static constexpr unsigned kStatsAt = kMeetRows * kPitch * 4, kUnitsAt = kStatsAt + kMeetRows * 8;
     static_assert(kUnitsAt + 2 * kTtM * 4 + 1024 <= kSmemBytes, "the results meet where queries and keys were");
     // Tensor memory of a team: scores of its even and odd blocks at columns 0 and 64, O from 128 on, the weights behind O at a
-    // head size of 64 and over the scores they were made of at 128.
-    static constexpr unsigned kTeamColumns = 256, kOColumn = 2 * kTtN;
-    static constexpr bool kOverScores = D == 128;
+    // head size of 64 and over the scores they were made of above.
+    static constexpr unsigned kTeamColumns = kAlone ? 0 : 256, kOColumn = 2 * kTtN;
+    static constexpr bool kOverScores = D > 64;
     static __device__ __forceinline__ unsigned p_column(int n) {
         return kOverScores ? (unsigned)((n & 1) * kTtN) : 2 * kTtN + D + (unsigned)((n & 1) * (kTtN / 2));
     }
@@ -230,9 +232,9 @@ __global__ void __launch_bounds__(kTtThreads, 1) attention_tree_tcgen05_kernel(c
     const int block_begin = all_begin + split * per_split;
     const int blocks = max(0, min(per_split, all_end - block_begin));
     // the team's n-th block is the piece's block kStride n + kFirst
-    constexpr int kStride = PAIRED ? 1 : 2;
-    const int first_block = PAIRED ? 0 : team;
-    const int mine = PAIRED ? blocks : (blocks + 1 - team) / 2;
+    constexpr int kStride = PAIRED || L::kAlone ? 1 : 2;
+    const int first_block = kStride == 1 ? 0 : team;
+    const int mine = PAIRED ? blocks : L::kAlone ? (team == 0 ? blocks : 0) : (blocks + 1 - team) / 2;
     const bool idle = PAIRED && team * kTtM >= rows;            // (a team without rows still gives its share of the stages back)
 
     const unsigned smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -562,7 +564,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) attention_tree_tcgen05_kernel(c
     // ---- what the teams have, of all pieces of the keys, meets in shared memory, where queries and keys were: every block of the
     // cluster owns some of the rows, and everybody writes a row's part (outputs, maximum, sum) to its owner
     const bool across = p.splits > 1 && p.part_o == nullptr;    // the pieces of the keys are a cluster
-    const int pieces = across ? p.splits : 1, parts = PAIRED ? pieces : 2 * pieces;
+    const int pieces = across ? p.splits : 1, parts = kStride == 1 ? pieces : 2 * pieces;
     const int row_first = across ? split * rows / p.splits : 0, count = (across ? (split + 1) * rows / p.splits : rows) - row_first;
     const int most = (rows + pieces - 1) / pieces;              // rows of an owner
     tcgen05_fence_before();
@@ -570,9 +572,9 @@ __global__ void __launch_bounds__(kTtThreads, 1) attention_tree_tcgen05_kernel(c
     if (across) cluster_sync();
     tcgen05_fence_after();
     const unsigned stats_at = smem_base + L::kStatsAt;          // [part][most] pairs; outputs before: [part][most][kPitch]
-    if (softmax && !idle) {
+    if (softmax && !idle && !(L::kAlone && team == 1)) {
         const int owner = across ? ((row + 1) * p.splits - 1) / rows : 0;
-        const int slot = (PAIRED ? (across ? split : 0) : (across ? 2 * split : 0) + team) * most + row - (across ? owner * rows / p.splits : 0);
+        const int slot = (kStride == 1 ? (across ? split : 0) : (across ? 2 * split : 0) + team) * most + row - (across ? owner * rows / p.splits : 0);
         const unsigned stats_to = peer_address(stats_at + (unsigned)slot * 8u, owner, across && live);
         const unsigned to = peer_address(smem_base + (unsigned)(slot * L::kPitch) * 4u, owner, across && live);
         if (live) store_2(stats_to, used_max, run_sum);
@@ -679,12 +681,12 @@ __global__ void __launch_bounds__(kTtThreads, 1) attention_tree_tcgen05_kernel(c
 
 bool tree_tcgen05_takes(const TreeParams& p) {
     // (page strides and (token, query head) numbers of 32 bits)
-    return p.head_dim % 8 == 0 && p.page_stride < (1ll << 32) && (long long)p.tokens * p.q_heads < (1ll << 31) && p.head_dim <= 128 && p.page_stride % 8 == 0 && p.q_row_stride % 8 == 0 && p.scale > 0.0f &&
+    return p.head_dim % 8 == 0 && p.head_dim <= 256 && p.page_stride < (1ll << 32) && (long long)p.tokens * p.q_heads < (1ll << 31) && p.page_stride % 8 == 0 && p.q_row_stride % 8 == 0 && p.scale > 0.0f &&
            (((size_t)p.q | (size_t)p.k_cache | (size_t)p.v_cache | (size_t)p.out | (size_t)p.part_o) & 15) == 0;
 }
 
 // Two teams' rows a tile where one tile of 128 does not hold them: the same keys would be read for every tile.
-static bool tree_paired(const TreeParams& p) { return p.max_nodes * p.group > kTtM; }
+static bool tree_paired(const TreeParams& p) { return p.head_dim <= 128 && p.max_nodes * p.group > kTtM; }
 
 // The kernel may have its shared memory: said once a device (a call of its own costs a small launch a tenth of its time).
 template <int D, bool PAIRED>
@@ -743,7 +745,8 @@ static TreeTile tree_tile() {
 
 TreeTile tree_tcgen05_tile(const TreeParams& p) {
     if (p.head_dim <= 64) return tree_paired(p) ? tree_tile<64, true>() : tree_tile<64, false>();
-    return tree_paired(p) ? tree_tile<128, true>() : tree_tile<128, false>();
+    if (p.head_dim <= 128) return tree_paired(p) ? tree_tile<128, true>() : tree_tile<128, false>();
+    return tree_tile<256, false>();
 }
 
 template <int D, bool PAIRED>
@@ -762,7 +765,8 @@ static int launch_tree(const TreeParams& p, cudaStream_t stream) {
 
 int launch_tree_tcgen05(const TreeParams& p, cudaStream_t stream) {
     if (p.head_dim <= 64) return tree_paired(p) ? launch_tree<64, true>(p, stream) : launch_tree<64, false>(p, stream);
-    return tree_paired(p) ? launch_tree<128, true>(p, stream) : launch_tree<128, false>(p, stream);
+    if (p.head_dim <= 128) return tree_paired(p) ? launch_tree<128, true>(p, stream) : launch_tree<128, false>(p, stream);
+    return launch_tree<256, false>(p, stream);
 }
 
 }  // namespace celeg_b200
