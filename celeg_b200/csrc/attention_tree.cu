@@ -14,6 +14,7 @@
 #include "attention_tree_tcgen05.h"
 #include "tcgen05.cuh"
 
+#include <cstring>
 #include <type_traits>
 
 namespace celeg_b200 {
@@ -386,18 +387,36 @@ static int tree_splits(long long problems, const TreeTile& tile, long long steps
 
 using namespace celeg_b200;
 
-// q: [tokens, q_row_stride] with head h at columns h * head_dim; caches: one layer's [pages, kv_heads, page_tokens, head_dim],
-// page_stride elements from page to page; span_begin [spans + 1], span_context [spans], ancestors [tokens, words] (words of 32
-// bits), block_table [spans, table_stride]; out [tokens, q_heads * head_dim]. max_nodes: no span has more nodes (error 4 else);
-// max_keys: about as many keys as the longest span has, which only the number of pieces follows. scratch: float32, any number
-// of elements; the keys are cut into no more pieces than it holds.
-CELEG_API int celeg_attention_tree(const void* q, long long q_row_stride, void* out, const void* k_cache, const void* v_cache,
-                                   long long page_stride, int pages, const int* positions, const int* span_begin,
-                                   const int* span_context, const int* ancestors, int words, const int* block_table,
-                                   int table_stride, int tokens, int spans, int max_nodes, int max_keys, int q_heads,
-                                   int kv_heads, int head_dim, int page_tokens, int window, float scale, const float* sinks,
-                                   float softcap, float* scratch, long long scratch_elements, int* error_flag, int act_dtype,
-                                   cudaStream_t stream) {
+// The arguments of the entry point, one record. q: [tokens, q_row_stride] with head h at columns h * head_dim; caches: one
+// layer's [pages, kv_heads, page_tokens, head_dim], page_stride elements from page to page; span_begin [spans + 1],
+// span_context [spans], ancestors [tokens, words] (words of 32 bits), block_table [spans, table_stride]; sinks [q_heads] or
+// null; out [tokens, q_heads * head_dim]. max_nodes: no span has more nodes (error 4 else); max_keys: about as many keys as the
+// longest span has, which only the number of pieces follows. scratch: float32, any number of elements; the keys are cut into
+// no more pieces than it holds where these do not meet in a cluster.
+struct TreeArguments {
+    const void *q;
+    void* out;
+    const void *k_cache, *v_cache;
+    const int *positions, *span_begin, *span_context, *ancestors, *block_table;
+    const float* sinks;
+    float* scratch;
+    int* error_flag;
+    cudaStream_t stream;
+    long long q_row_stride, page_stride, scratch_elements;
+    int pages, words, table_stride, tokens, spans, max_nodes, max_keys, q_heads, kv_heads, head_dim, page_tokens, window, act_dtype;
+    float scale, softcap;
+};
+static_assert(sizeof(TreeArguments) == 192, "the record that kernels.py packs");
+
+CELEG_API int celeg_attention_tree(const void* record) {
+    TreeArguments a;
+    memcpy(&a, record, sizeof(a));
+    const int tokens = a.tokens, spans = a.spans, max_nodes = a.max_nodes, max_keys = a.max_keys, q_heads = a.q_heads, kv_heads = a.kv_heads;
+    const int head_dim = a.head_dim, page_tokens = a.page_tokens, words = a.words, window = a.window, act_dtype = a.act_dtype;
+    const long long page_stride = a.page_stride;
+    const float scale = a.scale, softcap = a.softcap;
+    float* scratch = a.scratch;
+    cudaStream_t stream = a.stream;
     CELEG_REQUIRE(tokens >= 0 && spans >= 0 && q_heads > 0 && kv_heads > 0 && head_dim > 0 && page_tokens > 0 && max_keys >= 0,
                   "attention_tree: invalid sizes tokens=%d spans=%d q_heads=%d kv_heads=%d head_dim=%d page_tokens=%d", tokens,
                   spans, q_heads, kv_heads, head_dim, page_tokens);
@@ -406,8 +425,8 @@ CELEG_API int celeg_attention_tree(const void* q, long long q_row_stride, void* 
     CELEG_REQUIRE(max_nodes >= 1 && max_nodes <= kTreeMaxNodes && words >= (max_nodes + 31) / 32,
                   "attention_tree: trees of up to %d nodes (at most %d) need masks of %d words, got %d", max_nodes, kTreeMaxNodes,
                   (max_nodes + 31) / 32, words);
-    CELEG_REQUIRE(window >= 0 && softcap >= 0.0f && error_flag, "attention_tree: window %d, softcap %g, error_flag %p", window,
-                  softcap, (void*)error_flag);
+    CELEG_REQUIRE(window >= 0 && softcap >= 0.0f && a.error_flag, "attention_tree: window %d, softcap %g, error_flag %p", window,
+                  softcap, (void*)a.error_flag);
     CELEG_REQUIRE(act_dtype == kFloat32 || act_dtype == kBFloat16, "attention_tree: unknown dtype code %d", act_dtype);
     if (tokens == 0 || spans == 0) return 0;
     const int group = q_heads / kv_heads;
@@ -415,20 +434,20 @@ CELEG_API int celeg_attention_tree(const void* q, long long q_row_stride, void* 
     CELEG_REQUIRE(spans <= 65535 && kv_heads * tiles <= 65535 && (long long)max_nodes * group <= 1 << 24,
                   "attention_tree: %d spans of %d nodes on %d heads exceed one launch", spans, max_nodes, q_heads);
     TreeParams p = {};
-    p.q = q;
-    p.q_row_stride = q_row_stride;
-    p.out = out;
-    p.k_cache = k_cache;
-    p.v_cache = v_cache;
+    p.q = a.q;
+    p.q_row_stride = a.q_row_stride;
+    p.out = a.out;
+    p.k_cache = a.k_cache;
+    p.v_cache = a.v_cache;
     p.page_stride = page_stride;
-    p.pages = pages;
-    p.positions = positions;
-    p.span_begin = span_begin;
-    p.span_context = span_context;
-    p.ancestors = reinterpret_cast<const unsigned*>(ancestors);
+    p.pages = a.pages;
+    p.positions = a.positions;
+    p.span_begin = a.span_begin;
+    p.span_context = a.span_context;
+    p.ancestors = reinterpret_cast<const unsigned*>(a.ancestors);
     p.words = words;
-    p.block_table = block_table;
-    p.table_stride = table_stride;
+    p.block_table = a.block_table;
+    p.table_stride = a.table_stride;
     p.tokens = tokens;
     p.spans = spans;
     p.max_nodes = max_nodes;
@@ -442,20 +461,20 @@ CELEG_API int celeg_attention_tree(const void* q, long long q_row_stride, void* 
     for (int shift = 0; shift < 31; ++shift)
         if (page_tokens == 1 << shift) p.page_shift = shift;
     p.scale = scale;
-    p.sinks = sinks;
+    p.sinks = a.sinks;
     p.cap_in = softcap > 0.0f ? scale / softcap : 0.0f;
     p.cap_out = softcap;
-    p.error_flag = error_flag;
+    p.error_flag = a.error_flag;
     const long long units = (long long)tokens * q_heads;
     p.part_o = scratch;
     const bool tensor_cores = act_dtype == kBFloat16 && tree_tcgen05_takes(p);
     const size_t size = act_dtype == kFloat32 ? 4 : 2;
-    const bool pieces = head_dim * size % 16 == 0 && page_stride * size % 16 == 0 && (((size_t)k_cache | (size_t)v_cache) & 15) == 0;
+    const bool pieces = head_dim * size % 16 == 0 && page_stride * size % 16 == 0 && (((size_t)a.k_cache | (size_t)a.v_cache) & 15) == 0;
     TreeTile tile = {kSimtRows, 592, 2, 1, {0}};
     if (tensor_cores) tile = tree_tcgen05_tile(p);
     const long long reach = window > 0 && (long long)window + max_nodes < max_keys ? (long long)window + max_nodes : max_keys;
     p.splits = tree_splits((long long)spans * kv_heads * ((max_nodes * group + tile.rows - 1) / tile.rows), tile, (reach + 63) / 64,
-                           scratch ? scratch_elements / (units * (head_dim + 2)) : 0);
+                           scratch ? a.scratch_elements / (units * (head_dim + 2)) : 0);
     if (p.splits <= tile.cluster) p.part_o = nullptr;
     p.part_ml = p.part_o ? scratch + units * p.splits * head_dim : nullptr;
     int code;

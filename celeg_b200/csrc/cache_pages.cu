@@ -6,6 +6,7 @@
 #include "common.cuh"
 
 #include <cstdlib>
+#include <cstring>
 
 namespace celeg_b200 {
 
@@ -238,19 +239,26 @@ static CacheSide cache_side(void* base, long long layer_stride, long long page_s
     return {dim > 0 ? (unsigned char*)base : nullptr, layer_stride * element_bytes, page_stride * element_bytes, dim * element_bytes};
 }
 
-// k, v: [layers, pages, kv_heads, page_tokens, k_dim or v_dim], strides in elements, the last three sizes contiguous; a
-// dimension of 0: nothing is kept on that side. moves: `count` triples (from, to, rows) in host memory: the first `rows`
-// positions of page `to` become those of page `from`, in every layer. No page may be written twice, nor written and read
-// (a page onto itself aside): the moves run at the same time.
-CELEG_API int celeg_copy_pages(void* k, long long k_layer_stride, long long k_page_stride, int k_dim, void* v,
-                               long long v_layer_stride, long long v_page_stride, int v_dim, int layers, int pages, int kv_heads,
-                               int page_tokens, int element_bytes, const int* moves, int count, cudaStream_t stream) {
+// Both entry points take one record. Of the caches: k, v [layers, pages, kv_heads, page_tokens, k_dim or v_dim]; strides in
+// elements of keys' layers and pages and of values' layers and pages, the last three sizes contiguous; sizes k_dim, v_dim,
+// layers, pages, kv_heads, page_tokens, bytes of an element; a dimension of 0: nothing is kept on that side.
+
+// moves: `count` triples (from, to, rows) in host memory: the first `rows` positions of page `to` become those of page `from`, in
+// every layer. No page may be written twice, nor written and read (a page onto itself aside): the moves run at the same time.
+CELEG_API int celeg_copy_pages(const void* record) {
+    struct { void *k, *v; const int* moves; cudaStream_t stream; long long strides[4]; int sizes[7], count; } a;
+    static_assert(sizeof(a) == 96, "the record that kernels.py packs");
+    memcpy(&a, record, sizeof(a));
+    const int k_dim = a.sizes[0], v_dim = a.sizes[1], layers = a.sizes[2], pages = a.sizes[3], kv_heads = a.sizes[4];
+    const int page_tokens = a.sizes[5], element_bytes = a.sizes[6], count = a.count;
+    const int* moves = a.moves;
+    cudaStream_t stream = a.stream;
     CELEG_REQUIRE(layers > 0 && pages > 0 && kv_heads > 0 && page_tokens > 0 && k_dim >= 0 && v_dim >= 0 && count >= 0 &&
                       (element_bytes == 2 || element_bytes == 4),
                   "copy_pages: invalid sizes layers=%d pages=%d kv_heads=%d page_tokens=%d dims %d / %d count=%d element %d", layers,
                   pages, kv_heads, page_tokens, k_dim, v_dim, count, element_bytes);
-    const CacheSide ks = cache_side(k, k_layer_stride, k_page_stride, k_dim, element_bytes);
-    const CacheSide vs = cache_side(v, v_layer_stride, v_page_stride, v_dim, element_bytes);
+    const CacheSide ks = cache_side(a.k, a.strides[0], a.strides[1], k_dim, element_bytes);
+    const CacheSide vs = cache_side(a.v, a.strides[2], a.strides[3], v_dim, element_bytes);
     CELEG_REQUIRE(layers <= (1 << 30) / kManyMoves && (long long)kv_heads * page_tokens * (k_dim > v_dim ? k_dim : v_dim) * element_bytes < (1ll << 31),
                   "copy_pages: %d layers of pages of %d x %d x %d elements are too large", layers, kv_heads, page_tokens,
                   k_dim > v_dim ? k_dim : v_dim);
@@ -283,39 +291,47 @@ CELEG_API int celeg_copy_pages(void* k, long long k_layer_stride, long long k_pa
 
 // The accepted path of every span's tree: from node 0 on, the lowest child of the path's last node whose token is what the
 // model chose there. Rows at places context + path[n] move to context + n in every layer, keys and values.
-CELEG_API int celeg_keep_drafts(void* k, long long k_layer_stride, long long k_page_stride, int k_dim, void* v,
-                                long long v_layer_stride, long long v_page_stride, int v_dim, int layers, int pages, int kv_heads,
-                                int page_tokens, int element_bytes, const int* parents, const int* tokens, const int* chosen,
-                                int token_count, const int* span_begin, const int* span_context, const int* block_table,
-                                int table_stride, int spans, int max_nodes, int* path, int* accepted, int* next_token,
-                                int* error_flag, cudaStream_t stream) {
+CELEG_API int celeg_keep_drafts(const void* record) {
+    struct {
+        void *k, *v;
+        const int *parents, *tokens, *chosen, *span_begin, *span_context, *block_table;
+        int *path, *accepted, *next_token, *error_flag;
+        cudaStream_t stream;
+        long long strides[4];
+        int sizes[7], token_count, table_stride, spans, max_nodes;
+    } a;
+    static_assert(sizeof(a) == 184, "the record that kernels.py packs");
+    memcpy(&a, record, sizeof(a));
+    const int k_dim = a.sizes[0], v_dim = a.sizes[1], layers = a.sizes[2], pages = a.sizes[3], kv_heads = a.sizes[4];
+    const int page_tokens = a.sizes[5], element_bytes = a.sizes[6], token_count = a.token_count, spans = a.spans, max_nodes = a.max_nodes;
+    cudaStream_t stream = a.stream;
     CELEG_REQUIRE(layers > 0 && pages > 0 && kv_heads > 0 && page_tokens > 0 && k_dim >= 0 && v_dim >= 0 && token_count >= 0 &&
                       (element_bytes == 2 || element_bytes == 4),
                   "keep_drafts: invalid sizes layers=%d pages=%d kv_heads=%d page_tokens=%d dims %d / %d element %d", layers, pages,
                   kv_heads, page_tokens, k_dim, v_dim, element_bytes);
-    CELEG_REQUIRE(spans >= 0 && spans <= 65535 && max_nodes >= 1 && max_nodes <= kKeepMaxNodes && error_flag,
+    CELEG_REQUIRE(spans >= 0 && spans <= 65535 && max_nodes >= 1 && max_nodes <= kKeepMaxNodes && a.error_flag,
                   "keep_drafts: %d spans of up to %d nodes (at most 65535 and %d)", spans, max_nodes, kKeepMaxNodes);
     if (spans == 0) return 0;
     KeepParams p = {};
-    p.k = cache_side(k, k_layer_stride, k_page_stride, k_dim, element_bytes);
-    p.v = cache_side(v, v_layer_stride, v_page_stride, v_dim, element_bytes);
-    p.parents = parents;
-    p.tokens = tokens;
-    p.chosen = chosen;
-    p.span_begin = span_begin;
-    p.span_context = span_context;
-    p.block_table = block_table;
-    p.table_stride = table_stride;
+    p.k = cache_side(a.k, a.strides[0], a.strides[1], k_dim, element_bytes);
+    p.v = cache_side(a.v, a.strides[2], a.strides[3], v_dim, element_bytes);
+    p.parents = a.parents;
+    p.tokens = a.tokens;
+    p.chosen = a.chosen;
+    p.span_begin = a.span_begin;
+    p.span_context = a.span_context;
+    p.block_table = a.block_table;
+    p.table_stride = a.table_stride;
     p.pages = pages;
     p.token_count = token_count;
     p.layers = layers;
     p.kv_heads = kv_heads;
     p.page_tokens = page_tokens;
     p.max_nodes = max_nodes;
-    p.path = path;
-    p.accepted = accepted;
-    p.next_token = next_token;
-    p.error_flag = error_flag;
+    p.path = a.path;
+    p.accepted = a.accepted;
+    p.next_token = a.next_token;
+    p.error_flag = a.error_flag;
     const int piece = piece_bytes(p.k, p.v);
     if (piece == 16) launch_keep<uint4>(p, spans, stream);
     else if (piece == 8) launch_keep<uint2>(p, spans, stream);

@@ -18,6 +18,8 @@
 // Over many rows the logits' bytes are what bounds it; of few rows, the chain of a block's reductions.
 #include "common.cuh"
 
+#include <cstring>
+
 namespace celeg_b200 {
 
 constexpr int kLpThreads = 256;
@@ -483,30 +485,42 @@ static int launch_logprobs(const LogprobParams& p, int blocks, cudaStream_t stre
 
 using namespace celeg_b200;
 
-// logits: [rows, vocab] float32 or bfloat16, row_stride elements from row to row. tokens [rows] or null (no logprobs then);
-// entropy [rows] or null; top_logprobs and top_tokens [rows, top].
-CELEG_API int celeg_token_logprobs(const void* logits, long long row_stride, int rows, int vocab, const int* tokens,
-                                   float* logprobs, float* entropy, float* top_logprobs, int* top_tokens, int top,
-                                   int act_dtype, cudaStream_t stream) {
+// One record. logits: [rows, vocab] float32 or bfloat16, row_stride elements from row to row. tokens [rows] or null (no logprobs
+// then); entropy [rows] or null; top_logprobs and top_tokens [rows, top].
+CELEG_API int celeg_token_logprobs(const void* record) {
+    struct {
+        const void* logits;
+        const int* tokens;
+        float *logprobs, *entropy, *top_logprobs;
+        int* top_tokens;
+        cudaStream_t stream;
+        long long row_stride;
+        int rows, vocab, top, act_dtype;
+    } a;
+    static_assert(sizeof(a) == 80, "the record that kernels.py packs");
+    memcpy(&a, record, sizeof(a));
+    const int rows = a.rows, vocab = a.vocab, top = a.top, act_dtype = a.act_dtype;
+    const long long row_stride = a.row_stride;
+    cudaStream_t stream = a.stream;
     CELEG_REQUIRE(rows >= 0 && vocab > 0 && vocab < (1 << 30) && (rows <= 1 || row_stride >= vocab),
                   "token_logprobs: invalid sizes rows=%d vocab=%d row_stride=%lld", rows, vocab, row_stride);
-    CELEG_REQUIRE(top >= 0 && top <= kLpMaxTop && top <= vocab && (top == 0 || (top_logprobs && top_tokens)),
+    CELEG_REQUIRE(top >= 0 && top <= kLpMaxTop && top <= vocab && (top == 0 || (a.top_logprobs && a.top_tokens)),
                   "token_logprobs: %d alternatives (at most %d and the vocabulary of %d)", top, kLpMaxTop, vocab);
-    CELEG_REQUIRE(!logprobs || tokens, "token_logprobs: log probabilities of no tokens");
+    CELEG_REQUIRE(!a.logprobs || a.tokens, "token_logprobs: log probabilities of no tokens");
     CELEG_REQUIRE(act_dtype == kFloat32 || act_dtype == kBFloat16, "token_logprobs: unknown dtype code %d", act_dtype);
-    CELEG_REQUIRE(((size_t)logits & (act_dtype == kFloat32 ? 3 : 1)) == 0, "token_logprobs: logits at %p", logits);
+    CELEG_REQUIRE(((size_t)a.logits & (act_dtype == kFloat32 ? 3 : 1)) == 0, "token_logprobs: logits at %p", a.logits);
     if (rows == 0) return 0;
     LogprobParams p = {};
-    p.logits = logits;
+    p.logits = a.logits;
     p.row_stride = row_stride;
     p.rows = rows;
     p.vocab = vocab;
     p.top = top;
-    p.tokens = tokens;
-    p.logprobs = logprobs;
-    p.entropy = entropy;
-    p.top_logprobs = top_logprobs;
-    p.top_tokens = top_tokens;
+    p.tokens = a.tokens;
+    p.logprobs = a.logprobs;
+    p.entropy = a.entropy;
+    p.top_logprobs = a.top_logprobs;
+    p.top_tokens = a.top_tokens;
     // few rows: up to eight blocks a row, as long as a block has 4,096 logits and the blocks fit on the GPU together
     int blocks = 1;
     while (blocks < kLpMaxBlocks && (long long)rows * blocks * 2 <= 592 && vocab / (blocks * 2) >= 4096) blocks *= 2;

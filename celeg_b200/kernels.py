@@ -9,7 +9,8 @@ from __future__ import annotations
 
 import ctypes
 import functools
-from ctypes import c_float, c_int, c_longlong, c_void_p
+import struct
+from ctypes import c_char_p, c_float, c_int, c_longlong, c_void_p
 from typing import Optional, Tuple
 
 import numpy as np
@@ -204,16 +205,10 @@ _SIGNATURES = {
     "celeg_scalar_decay_decode": [c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p,
                                   c_void_p, c_void_p, c_longlong, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p,
                                   c_void_p],
-    "celeg_attention_tree": [c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_longlong, c_int, c_void_p, c_void_p, c_void_p,
-                             c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
-                             c_float, c_void_p, c_float, c_void_p, c_longlong, c_void_p, c_int, c_void_p],
-    "celeg_copy_pages": [c_void_p, c_longlong, c_longlong, c_int, c_void_p, c_longlong, c_longlong, c_int, c_int, c_int, c_int,
-                         c_int, c_int, c_void_p, c_int, c_void_p],
-    "celeg_keep_drafts": [c_void_p, c_longlong, c_longlong, c_int, c_void_p, c_longlong, c_longlong, c_int, c_int, c_int, c_int,
-                          c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
-                          c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
-    "celeg_token_logprobs": [c_void_p, c_longlong, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
-                             c_void_p],
+    "celeg_attention_tree": [c_char_p],
+    "celeg_copy_pages": [c_char_p],
+    "celeg_keep_drafts": [c_char_p],
+    "celeg_token_logprobs": [c_char_p],
     "celeg_moe_combine": [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
                           c_void_p],
 }
@@ -853,6 +848,25 @@ TREE_MAX_HEAD_DIM = 256
 MAX_TOP_LOGPROBS = 128
 
 
+# The arguments of these entry points travel as one record (ctypes takes 3.4 us for thirty of them, a record 0.7): addresses
+# and 64-bit numbers first, then 32-bit ones, as the structs of csrc/attention_tree.cu, cache_pages.cu and logprobs.cu have them.
+_TREE_RECORD = struct.Struct("=13Q3q13i2f4x")
+_COPY_RECORD = struct.Struct("=4Q4q8i")
+_KEEP_RECORD = struct.Struct("=13Q4q11i4x")
+_LOGPROBS_RECORD = struct.Struct("=7Qq4i")
+
+
+def _record(operator: str, layout: struct.Struct, *values) -> bytes:
+    try:
+        return layout.pack(*values)
+    except struct.error as exc:
+        raise KernelLibraryError(f"{operator}: an argument is not a number of its kind: {exc}") from exc
+
+
+def _address(tensor: Optional[torch.Tensor]) -> int:
+    return 0 if tensor is None else tensor.data_ptr()
+
+
 def _refuse(what: str) -> None:
     raise KernelLibraryError(what)
 
@@ -936,12 +950,12 @@ def attention_tree(q: torch.Tensor, q_row_stride: int, out: torch.Tensor, k_cach
         _check_vectors(name, device, (("sinks", sinks, q_heads, torch.float32),))
     if scratch is not None and (scratch.dtype is not torch.float32 or not scratch.is_contiguous() or scratch.get_device() != device):
         _check_vectors(name, device, (("scratch", scratch, 0, torch.float32),))
-    _check(library().celeg_attention_tree(
-        q.data_ptr(), q_row_stride, out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), strides[0], shape[0],
-        positions.data_ptr(), span_begin.data_ptr(), span_context.data_ptr(), ancestors.data_ptr(), masks[1],
-        block_table.data_ptr(), block_table.stride(0), tokens, spans, max_nodes, max_keys, q_heads, kv_heads, head_dim,
-        page_tokens, int(window or 0), scale, _ptr(sinks), float(softcap or 0.0), _ptr(scratch),
-        scratch.numel() if scratch is not None else 0, error_flag.data_ptr(), code, _stream()))
+    _check(library().celeg_attention_tree(_record(
+        name, _TREE_RECORD, q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), positions.data_ptr(),
+        span_begin.data_ptr(), span_context.data_ptr(), ancestors.data_ptr(), block_table.data_ptr(), _address(sinks),
+        _address(scratch), error_flag.data_ptr(), _stream(), q_row_stride, strides[0], scratch.numel() if scratch is not None else 0,
+        shape[0], masks[1], block_table.stride(0), tokens, spans, max_nodes, max_keys, q_heads, kv_heads, head_dim, page_tokens,
+        window or 0, code, scale, softcap or 0.0)))
 
 
 def _cache_sides(operator: str, k: torch.Tensor, v: torch.Tensor) -> tuple:
@@ -958,8 +972,8 @@ def _cache_sides(operator: str, k: torch.Tensor, v: torch.Tensor) -> tuple:
                 f"and {v_strides} of {tuple(v_shape)}")
     if k.get_device() != v.get_device():
         _refuse(f"{operator}: keys on {k.device}, values on {v.device}")
-    return (k.data_ptr(), k_strides[0], k_strides[1], k_dim, v.data_ptr(), v_strides[0], v_strides[1], v_dim, layers, pages,
-            heads, page_tokens, element)
+    return k.data_ptr(), v.data_ptr(), (k_strides[0], k_strides[1], v_strides[0], v_strides[1], k_dim, v_dim, layers, pages, heads,
+                                        page_tokens, element)
 
 
 def copy_pages(k: torch.Tensor, v: torch.Tensor, moves) -> None:
@@ -967,7 +981,7 @@ def copy_pages(k: torch.Tensor, v: torch.Tensor, moves) -> None:
     array of (from, to, positions): the first ``positions`` of page ``to`` become those of page ``from`` in every layer, what
     lies behind them stays. A page may be read by many moves; none may be written twice, or written by one and read by
     another. ``k``, ``v``: [layers, pages, kv_heads, page_tokens, *]."""
-    sides = _cache_sides("copy_pages", k, v)
+    keys, values, sizes = _cache_sides("copy_pages", k, v)
     table = moves if isinstance(moves, np.ndarray) else np.asarray(moves)
     if table.size == 0:
         return
@@ -979,7 +993,8 @@ def copy_pages(k: torch.Tensor, v: torch.Tensor, moves) -> None:
         table = table.astype(np.int32)
     table = np.ascontiguousarray(table)
     _check_vectors("copy_pages", k.get_device(), ())
-    _check(library().celeg_copy_pages(*sides, table.__array_interface__["data"][0], table.shape[0], _stream()))
+    _check(library().celeg_copy_pages(_record("copy_pages", _COPY_RECORD, keys, values, table.__array_interface__["data"][0], _stream(),
+                                              *sizes, table.shape[0])))
 
 
 def keep_drafts(k: torch.Tensor, v: torch.Tensor, parents: torch.Tensor, tokens: torch.Tensor, chosen: torch.Tensor,
@@ -993,7 +1008,7 @@ def keep_drafts(k: torch.Tensor, v: torch.Tensor, parents: torch.Tensor, tokens:
     ``accepted`` [spans] (its length) and ``next_token`` [spans] (what was chosen after its last node). A span without nodes:
     0 and -1. ``k``, ``v``: as for :func:`copy_pages`; a span's table row and places as for :func:`attention_tree`."""
     name = "keep_drafts"
-    sides = _cache_sides(name, k, v)
+    keys, values, sizes = _cache_sides(name, k, v)
     count = min(parents.numel(), tokens.numel(), chosen.numel())
     _check_table(name, block_table, spans)
     device = k.get_device()
@@ -1013,10 +1028,10 @@ def keep_drafts(k: torch.Tensor, v: torch.Tensor, parents: torch.Tensor, tokens:
             ("span_begin", span_begin, spans + 1, _I32), ("span_context", span_context, spans, _I32),
             ("path", path, spans * max_nodes, _I32), ("accepted", accepted, spans, _I32), ("next_token", next_token, spans, _I32),
             ("error_flag", error_flag, 1, _I32)))
-    _check(library().celeg_keep_drafts(
-        *sides, parents.data_ptr(), tokens.data_ptr(), chosen.data_ptr(), count, span_begin.data_ptr(), span_context.data_ptr(),
-        block_table.data_ptr(), block_table.stride(0), spans, max_nodes, path.data_ptr(), accepted.data_ptr(),
-        next_token.data_ptr(), error_flag.data_ptr(), _stream()))
+    _check(library().celeg_keep_drafts(_record(
+        name, _KEEP_RECORD, keys, values, parents.data_ptr(), tokens.data_ptr(), chosen.data_ptr(), span_begin.data_ptr(),
+        span_context.data_ptr(), block_table.data_ptr(), path.data_ptr(), accepted.data_ptr(), next_token.data_ptr(),
+        error_flag.data_ptr(), _stream(), *sizes, count, block_table.stride(0), spans, max_nodes)))
 
 
 def token_logprobs(logits: torch.Tensor, rows: int, tokens: Optional[torch.Tensor], logprobs: Optional[torch.Tensor],
@@ -1050,9 +1065,9 @@ def token_logprobs(logits: torch.Tensor, rows: int, tokens: Optional[torch.Tenso
     elif top_tokens is not None or top_logprobs is not None:
         _refuse(f"{name}: top_logprobs and top_tokens come together")
     _check_vectors(name, logits.get_device(), vectors)
-    _check(library().celeg_token_logprobs(
-        logits.data_ptr(), logits.stride(0), rows, vocab, _ptr(tokens), _ptr(logprobs), _ptr(entropy), _ptr(top_logprobs),
-        _ptr(top_tokens), top, code, _stream()))
+    _check(library().celeg_token_logprobs(_record(
+        name, _LOGPROBS_RECORD, logits.data_ptr(), _address(tokens), _address(logprobs), _address(entropy), _address(top_logprobs),
+        _address(top_tokens), _stream(), logits.stride(0), rows, vocab, top, code)))
 
 
 # ------------------------------------------------------- Dynamic Tanh blocks, matrix-state mixers

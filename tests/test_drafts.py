@@ -80,9 +80,9 @@ def test_the_library_refuses_sizes():
     def tree(**changes):
         a = dict(tokens=5, spans=2, max_nodes=3, max_keys=9, q_heads=4, kv_heads=2, head_dim=64, page_tokens=16, window=0, words=1, softcap=0.0, dtype=0)
         a.update(changes)
-        return lib.celeg_attention_tree(None, 256, None, None, None, 2048, 4, None, None, None, None, a["words"], None, 2, a["tokens"], a["spans"],
-                                        a["max_nodes"], a["max_keys"], a["q_heads"], a["kv_heads"], a["head_dim"], a["page_tokens"], a["window"], 0.1,
-                                        None, a["softcap"], None, 0, 1, a["dtype"], None)
+        return lib.celeg_attention_tree(kernels._TREE_RECORD.pack(
+            *[0] * 11, 1, 0, 256, 2048, 0, 4, a["words"], 2, a["tokens"], a["spans"], a["max_nodes"], a["max_keys"], a["q_heads"], a["kv_heads"],
+            a["head_dim"], a["page_tokens"], a["window"], a["dtype"], 0.1, a["softcap"]))
     for changes in (dict(q_heads=5), dict(head_dim=257), dict(head_dim=0), dict(max_nodes=257, words=9), dict(max_nodes=33), dict(max_nodes=0),
                     dict(tokens=-1), dict(spans=-1), dict(window=-2), dict(softcap=-1.0), dict(dtype=7), dict(spans=70000), dict(page_tokens=0)):
         assert tree(**changes) == -1, changes
@@ -90,7 +90,7 @@ def test_the_library_refuses_sizes():
     moves = np.array([[0, 4, 1]], dtype=np.int32)
 
     def copy(pages=5, element=4, count=1, dim=8):
-        return lib.celeg_copy_pages(16, 100, 20, dim, 16, 100, 20, 8, 2, pages, 1, 4, element, moves.ctypes.data, count, None)
+        return lib.celeg_copy_pages(kernels._COPY_RECORD.pack(16, 16, moves.ctypes.data, 0, 100, 20, 100, 20, dim, 8, 2, pages, 1, 4, element, count))
     for clash in ([[0, 1, 4], [2, 1, 4]], [[0, 1, 4], [1, 2, 4]], [[3, 3, 1], [3, 4, 1]]):
         moves = np.array(clash, dtype=np.int32)
         assert copy(count=2) == -1 and b"another" in lib.celeg_last_error()
@@ -100,11 +100,18 @@ def test_the_library_refuses_sizes():
     assert copy(pages=4) == -1 and copy(element=1) == -1 and copy(dim=-1) == -1 and copy(count=-1) == -1 and copy(count=0) == 0
 
     def keep(max_nodes=4, spans=1, element=2):
-        return lib.celeg_keep_drafts(16, 100, 20, 8, 16, 100, 20, 8, 2, 5, 1, 4, element, None, None, None, 6, None, None, None, 3, spans, max_nodes,
-                                     None, None, None, 1, None)
+        return lib.celeg_keep_drafts(kernels._KEEP_RECORD.pack(16, 16, *[0] * 9, 1, 0, 100, 20, 100, 20, 8, 8, 2, 5, 1, 4, element, 6, 3, spans,
+                                                               max_nodes))
     assert keep(max_nodes=257) == -1 and keep(max_nodes=0) == -1 and keep(spans=-1) == -1 and keep(element=3) == -1 and keep(spans=0) == 0
 
     def logprobs(rows=2, vocab=10, top=0, stride=10, dtype=0, at=16):
-        return lib.celeg_token_logprobs(at, stride, rows, vocab, None, None, None, 16, 16, top, dtype, None)
+        return lib.celeg_token_logprobs(kernels._LOGPROBS_RECORD.pack(at, 0, 0, 0, 16, 16, 0, stride, rows, vocab, top, dtype))
     assert logprobs(vocab=0) == -1 and logprobs(top=11) == -1 and logprobs(stride=9) == -1 and logprobs(dtype=3) == -1 and logprobs(at=18) == -1
     assert logprobs(rows=-1) == -1 and logprobs(vocab=500, stride=500, top=129) == -1 and logprobs(rows=0) == 0
+
+
+def test_numbers_that_do_not_fit_their_kind_are_refused():
+    with pytest.raises(KernelLibraryError, match="not a number of its kind"):
+        kernels._record("attention_tree", kernels._TREE_RECORD, *[0] * 13, 0, 0, 0, 1 << 31, *[0] * 12, 0.0, 0.0)
+    with pytest.raises(KernelLibraryError, match="not a number of its kind"):
+        kernels._record("token_logprobs", kernels._LOGPROBS_RECORD, *[0] * 8, 1.5, 0, 0, 0)
