@@ -415,7 +415,10 @@ CELEG_API int celeg_attention_tree(const void* record) {
     const int head_dim = a.head_dim, page_tokens = a.page_tokens, words = a.words, window = a.window, act_dtype = a.act_dtype;
     const long long page_stride = a.page_stride;
     const float scale = a.scale, softcap = a.softcap;
-    float* scratch = a.scratch;
+    // (scratch is used from a 16-byte address on)
+    const long long skipped = (long long)((16 - ((size_t)a.scratch & 15)) & 15) / 4;
+    float* scratch = a.scratch && a.scratch_elements > skipped ? a.scratch + skipped : nullptr;
+    const long long scratch_elements = scratch ? a.scratch_elements - skipped : 0;
     cudaStream_t stream = a.stream;
     CELEG_REQUIRE(tokens >= 0 && spans >= 0 && q_heads > 0 && kv_heads > 0 && head_dim > 0 && page_tokens > 0 && max_keys >= 0,
                   "attention_tree: invalid sizes tokens=%d spans=%d q_heads=%d kv_heads=%d head_dim=%d page_tokens=%d", tokens,
@@ -474,9 +477,9 @@ CELEG_API int celeg_attention_tree(const void* record) {
     if (tensor_cores) tile = tree_tcgen05_tile(p);
     const long long reach = window > 0 && (long long)window + max_nodes < max_keys ? (long long)window + max_nodes : max_keys;
     p.splits = tree_splits((long long)spans * kv_heads * ((max_nodes * group + tile.rows - 1) / tile.rows), tile, (reach + 63) / 64,
-                           scratch ? a.scratch_elements / (units * (head_dim + 2)) : 0);
+                           scratch ? (scratch_elements - 1) / (units * (head_dim + 2)) : 0);
     if (p.splits <= tile.cluster) p.part_o = nullptr;
-    p.part_ml = p.part_o ? scratch + units * p.splits * head_dim : nullptr;
+    p.part_ml = p.part_o ? scratch + (units * p.splits * head_dim + 1) / 2 * 2 : nullptr;      // (read as pairs)
     int code;
     if (tensor_cores)
         code = launch_tree_tcgen05(p, stream);

@@ -15,6 +15,7 @@
 namespace celeg_b200 {
 
 constexpr int kTreeMaxNodes = 256;            // masks are read in words of 32 nodes, eight at most
+constexpr long long kTreeMaxPlaces = 0x7fffffffll - 1024;      // a block of keys behind the last place still has a 32-bit number
 
 struct TreeParams {
     const void* q;                 // [tokens, q_row_stride], head h at h * head_dim
@@ -39,7 +40,8 @@ struct TreeParams {
     int* error_flag;
 };
 
-// One span as a block sees it; nodes 0 where the block has nothing to do.
+// One span as a block sees it; nodes 0 where the block has nothing to do, or must not begin: a span outside the launch's sizes
+// (error 4), or with places behind its row of the table (error 2), whose rows are left as they were.
 struct TreeSpan {
     int begin, nodes, context;
 };
@@ -51,6 +53,11 @@ __device__ __forceinline__ TreeSpan tree_span(const TreeParams& p, int span) {
     s.context = p.span_context[span];
     if (s.begin < 0 || s.nodes < 0 || s.begin > p.tokens - s.nodes || s.nodes > p.max_nodes || s.context < 0) {
         if (s.nodes != 0) atomicExch(p.error_flag, 4);
+        s.nodes = 0;
+    }
+    const long long places = (long long)p.table_stride * p.page_tokens;
+    if (s.nodes > 0 && (long long)s.context + s.nodes > (places < kTreeMaxPlaces ? places : kTreeMaxPlaces)) {
+        atomicExch(p.error_flag, 2);
         s.nodes = 0;
     }
     return s;

@@ -136,8 +136,16 @@ __global__ void __launch_bounds__(kKeepThreads) keep_drafts_kernel(const KeepPar
     __shared__ int accepted_s, moved_s;
     const int span = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
     const int begin = p.span_begin[span], nodes = p.span_begin[span + 1] - begin, context = p.span_context[span];
-    if (begin < 0 || nodes < 0 || begin > p.token_count - nodes || nodes > p.max_nodes || context < 0) {
-        if (tid == 0) atomicExch(p.error_flag, 4);
+    if (begin < 0 || nodes < 0 || begin > p.token_count - nodes || nodes > p.max_nodes || context < 0 ||
+        context > 0x7fffffff - kKeepMaxNodes) {
+        if (blockIdx.x == 0) {
+            for (int n = tid; n < p.max_nodes; n += kKeepThreads) p.path[(size_t)span * p.max_nodes + n] = -1;
+            if (tid == 0) {
+                p.accepted[span] = 0;
+                p.next_token[span] = -1;
+                atomicExch(p.error_flag, 4);
+            }
+        }
         return;
     }
     if (tid < 32) {

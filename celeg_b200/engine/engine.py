@@ -258,6 +258,8 @@ class Engine:
         token behind the first, given those before it, the entropy of the distribution it was taken from and, with
         ``top`` (at most 128), the most likely tokens there. One prompt gives one, several give a list. Needs a free
         state slot and pages for one prompt at a time; unscaled logits (temperature 1, no penalties)."""
+        if isinstance(prompts, (np.ndarray, torch.Tensor)):
+            prompts = prompts.tolist()
         single = len(prompts) > 0 and not isinstance(prompts[0], (list, tuple, np.ndarray, torch.Tensor))
         batch = [prompts] if single else list(prompts)
         vocab = self.loaded.model.vocab_size

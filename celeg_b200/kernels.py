@@ -911,7 +911,8 @@ def attention_tree(q: torch.Tensor, q_row_stride: int, out: torch.Tensor, k_cach
     positions and, behind them, node j at place span_context[s] + j (keys and values already stored). A node sees the cached
     positions and the nodes whose bits its row of ``ancestors`` has (int32 [tokens, words], bit j % 32 of word j // 32; a node
     sees itself only with its own bit), of these under a ``window`` those less than that many positions before its own:
-    ``positions`` [tokens] are the nodes' positions, a cached place's is itself. A row that sees nothing is zeros.
+    ``positions`` [tokens] are the nodes' positions, a cached place's is itself. A row that sees nothing is zeros. Rows behind the last
+    span, and of a span that reaches past its row of the table (error 2) or the launch's sizes (error 4), stay as they were.
     ``q`` [tokens, *] with head h at column h * head_dim, rows ``q_row_stride`` apart; ``out`` [tokens, q_heads * head_dim];
     caches: one layer's pages. ``sinks``, ``softcap``: as for :func:`attention_generic`. ``max_keys``: about the longest span's
     cached positions and nodes; with ``scratch`` (:func:`attention_tree_scratch`, or any float32 vector) long contexts are cut
@@ -1005,8 +1006,8 @@ def keep_drafts(k: torch.Tensor, v: torch.Tensor, parents: torch.Tensor, tokens:
     the lowest where several are, and ends where none is. ``parents`` [tokens]: a node's parent within its span, below the node
     itself; -1 for node 0. The path's keys and values move from places span_context[s] + path[n] to span_context[s] + n, in
     every layer, so that they are the next cached positions. Written: ``path`` [spans, max_nodes] (-1 behind the path),
-    ``accepted`` [spans] (its length) and ``next_token`` [spans] (what was chosen after its last node). A span without nodes:
-    0 and -1. ``k``, ``v``: as for :func:`copy_pages`; a span's table row and places as for :func:`attention_tree`."""
+    ``accepted`` [spans] (its length) and ``next_token`` [spans] (what was chosen after its last node). A span without nodes,
+    or one that is refused (error 4): 0 and -1. ``k``, ``v``: as for :func:`copy_pages`; a span's table row and places as for :func:`attention_tree`."""
     name = "keep_drafts"
     keys, values, sizes = _cache_sides(name, k, v)
     count = min(parents.numel(), tokens.numel(), chosen.numel())

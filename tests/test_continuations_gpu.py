@@ -109,6 +109,17 @@ def test_score(tmp_path, name, dtype):
     assert all(group.pool.used_pages == 0 for group in engine.loaded.manager.groups)
 
 
+def test_score_takes_arrays(tmp_path):
+    engine = engine_of(tmp_path, "A", "float32")
+    prompt = [3, 1, 4, 1, 5, 9, 2, 6]
+    want = engine.score(prompt).logprobs
+    for one in (tuple(prompt), np.array(prompt), torch.tensor(prompt), torch.tensor(prompt, device="cuda")):
+        assert engine.score(one).logprobs == want
+    for several in ([np.array(prompt), torch.tensor(prompt)], np.array([prompt] * 2), torch.tensor([prompt] * 2)):
+        assert [scores.logprobs for scores in engine.score(several)] == [want] * 2
+    assert engine.score([]) == []
+
+
 def test_score_in_portions(tmp_path, monkeypatch):
     from celeg_b200.engine import engine as module
     engine = engine_of(tmp_path, "B", "float32")

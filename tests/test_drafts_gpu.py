@@ -56,13 +56,15 @@ class Trees:
                                        self.positions[s], c, scale, window, sinks, softcap)
         return out
 
-    def run(self, scale, window=0, sinks=None, softcap=0.0, scratch=None, out=None, q=None, stream=None, max_keys=None):
+    def run(self, scale, window=0, sinks=None, softcap=0.0, scratch=None, out=None, q=None, max_keys=None, k=None, v=None,
+            table=None):
         from celeg_b200 import kernels
         out = torch.full((self.total + 2, self.heads * self.dim), 7.0, dtype=self.dtype, device="cuda") if out is None else out
         flag = torch.zeros(1, dtype=I32, device="cuda")
         q = self.q.cuda() if q is None else q
-        kernels.attention_tree(q, q.stride(0), out, self.k.cuda(), self.v.cuda(), i32(np.concatenate(self.positions)),
-                               i32(self.begin), i32(self.context), i32(self.masks), i32(self.table), self.total, len(self.spans),
+        k, v = (self.k.cuda(), self.v.cuda()) if k is None else (k, v)
+        kernels.attention_tree(q, q.stride(0), out, k, v, i32(np.concatenate(self.positions)), i32(self.begin), i32(self.context),
+                               i32(self.masks), i32(self.table) if table is None else table, self.total, len(self.spans),
                                self.max_nodes, max_keys if max_keys is not None else max(n + c for n, c in self.spans), self.heads,
                                self.kv_heads, self.dim, self.page, window, scale, scratch, flag,
                                sinks=None if sinks is None else torch.tensor(sinks, dtype=torch.float32, device="cuda"), softcap=softcap)
@@ -263,6 +265,158 @@ def test_tree_attention_same_bits_again_on_another_stream_and_in_a_graph():
     assert torch.equal(out[:t.total], first[:t.total])
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dim", [33, 34, 64])
+def test_tree_attention_scratch_of_any_size_and_address(dim, dtype):
+    """Odd numbers of pieces of odd heads, scratch that begins anywhere and holds hardly anything."""
+    from celeg_b200 import kernels
+    whole = kernels.attention_tree_scratch("cuda")
+    for context in (130, 330, 500, 700):
+        t = Trees([(1, context)], 1, 1, dim, 16, dtype, seed=context)
+        want = t.want(0.2)
+        for offset, size in ((0, 1 << 20), (1, 1 << 20), (2, 1 << 20), (3, 200), (1, 3), (2, 0), (1, 3 * (dim + 2)), (0, 5 * (dim + 2))):
+            out, flag = t.run(0.2, scratch=whole[offset:offset + size])
+            assert flag == 0
+            t.check(out, want)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("page", [1, 3, 8, 64, 128, 256])
+def test_tree_attention_pages_of_all_sizes(page, dim):
+    t = Trees([(5, 2100), (40, 700), (2, 63)], 4, 2, dim, page, torch.bfloat16, seed=page + dim)
+    out, flag = t.run(dim ** -0.5)
+    assert flag == 0
+    t.check(out, t.want(dim ** -0.5))
+    t.table[0, 3] = t.pages                                  # a page that is missing is reported by all forms
+    assert t.run(dim ** -0.5)[1] == 2
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("window,sinks,softcap", [(0, True, 0.0), (33, False, 0.0), (500, True, 30.0)])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(16, 2, 64), (16, 2, 128), (16, 1, 80), (16, 2, 256), (12, 2, 136)])
+def test_tree_attention_of_many_rows(heads, kv_heads, dim, window, sinks, softcap, dtype):
+    """More rows than a tile of either size, the last one nearly empty."""
+    t = Trees([(40, 500), (33, 0), (17, 129)], heads, kv_heads, dim, 16, dtype, seed=window + dim)
+    values = t.rng.normal(size=heads).astype(np.float32) if sinks else None
+    if window:
+        for s, c in enumerate(t.context):
+            t.table[s, :max(0, c - window + 1) // 16] = -1
+    out, flag = t.run(dim ** -0.5, window, values, softcap)
+    assert flag == 0
+    t.check(out, t.want(dim ** -0.5, window, values, softcap))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("heads,dim,nodes", [(4, 64, 3), (4, 128, 3), (2, 256, 5), (4, 72, 3), (32, 64, 8), (32, 128, 8)])
+def test_tree_attention_of_few_rows_over_many_positions(heads, dim, nodes, dtype):
+    """Cut into more pieces than a cluster holds; and into as many as it holds, or as scratch does."""
+    from celeg_b200 import kernels
+    t = Trees([(nodes, 20011)], heads, 1, dim, 16, dtype, seed=dim + heads)
+    values = t.rng.normal(size=heads).astype(np.float32)
+    want = t.want(dim ** -0.5, 0, values)
+    for scratch in (None, kernels.attention_tree_scratch("cuda"), torch.empty(11 * t.total * heads * (dim + 2), device="cuda")):
+        out, flag = t.run(dim ** -0.5, 0, values, scratch=scratch)
+        assert flag == 0
+        t.check(out, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_tree_attention_of_256_nodes_and_of_many_spans(dtype):
+    t = Trees([(256, 300), (1, 5)], 4, 2, 64, 16, dtype, seed=1, words=11)
+    out, flag = t.run(0.125)
+    assert flag == 0
+    t.check(out, t.want(0.125))
+    t = Trees([(i % 3, i % 41) for i in range(400)], 4, 2, 64, 16, dtype, seed=2)
+    out, flag = t.run(0.125, max_keys=0)                     # (max_keys is a hint)
+    assert flag == 0
+    t.check(out, t.want(0.125))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_tree_attention_strides_and_shared_pages(dim, dtype):
+    """Queries at odd addresses, a table that is part of a wider one, caches that are part of larger pages; and two spans that
+    share their first pages."""
+    t = Trees([(12, 200), (9, 230)], 4, 2, dim, 16, dtype, seed=4)
+    t.table[1, :12] = t.table[0, :12]
+    want = t.want(0.1)
+    wide_q = torch.zeros((t.total, t.q.shape[1] + 5), dtype=dtype, device="cuda")
+    wide_table = torch.full((2, t.table.shape[1] + 7), -1, dtype=I32, device="cuda")
+    wide_table[:, 3:3 + t.table.shape[1]] = i32(t.table)
+    large_k, large_v = (torch.full((t.pages, 5, 16, dim), float("nan"), dtype=dtype, device="cuda") for _ in range(2))
+    large_k[:, 1:3], large_v[:, 1:3] = t.k.cuda(), t.v.cuda()
+    for offset in (0, 1, 4, 5):
+        q = wide_q[:, offset:offset + t.q.shape[1]]
+        q.copy_(t.q)
+        out, flag = t.run(0.1, q=q, table=wide_table[:, 3:], k=large_k[:, 1:3], v=large_v[:, 1:3])
+        assert flag == 0
+        t.check(out, want)
+
+
+def test_tree_attention_contexts_past_the_table_are_refused():
+    """... with their rows left alone, and nothing behind the table read, whatever the context is."""
+    for dtype in (torch.float32, torch.bfloat16):
+        t = Trees([(6, 40), (4, 20)], 4, 1, 64, 16, dtype, seed=1)
+        good, _ = t.run(0.125)
+        places = t.table.shape[1] * 16
+        for context in (places - 5, places, 1 << 30, 2 ** 31 - 1100, 2 ** 31 - 300, 2 ** 31 - 2, 2 ** 31 - 1):
+            t.context = [context, 20]
+            out, flag = t.run(0.125)
+            assert flag == 2 and torch.equal(out[6:10], good[6:10]) and bool((out[:6] == 7.0).all())
+
+
+def test_tree_attention_two_calls_at_once():
+    from celeg_b200 import kernels
+    t = Trees([(9, 20011)], 4, 1, 64, 16, torch.bfloat16, seed=2)
+    scratch = [kernels.attention_tree_scratch("cuda") for _ in range(2)]
+    want, _ = t.run(0.125, scratch=scratch[0])
+    q, k, v = t.q.cuda(), t.k.cuda(), t.v.cuda()
+    fixed = [i32(np.concatenate(t.positions)), i32(t.begin), i32(t.context), i32(t.masks), i32(t.table)]
+    flag = torch.zeros(1, dtype=I32, device="cuda")
+    outs = [torch.zeros((9, 256), dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for stream, out, own in zip(streams, outs, scratch):
+            with torch.cuda.stream(stream):
+                kernels.attention_tree(q, q.stride(0), out, k, v, *fixed, 9, 1, 9, 20020, 4, 1, 64, 16, None, 0.125, own, flag)
+    torch.cuda.synchronize()
+    assert int(flag.item()) == 0
+    for out in outs:
+        assert torch.equal(out, want[:9])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_caches_larger_than_32_bit_offsets(dtype):
+    """Pages behind the first 2^32 elements: read by attention, moved by keep_drafts, copied."""
+    from celeg_b200 import kernels
+    t = Trees([(12, 200), (9, 1300)], 16, 8, 64, 16, dtype, seed=6)
+    per_page = 8 * 16 * 64
+    pages = (1 << 32) // per_page + t.pages + 100
+    large = [torch.empty((1, pages, 8, 16, 64), dtype=dtype, device="cuda") for _ in range(2)]
+    at = pages - t.pages
+    large[0][0, at:], large[1][0, at:] = t.k.cuda(), t.v.cuda()
+    table = i32(np.where(t.table >= 0, t.table + at, -1))
+    want, _ = t.run(0.125)
+    got, flag = t.run(0.125, k=large[0][0], v=large[1][0], table=table)
+    assert flag == 0 and torch.equal(got, want)
+    small = [t.k.cuda()[None].clone(), t.v.cuda()[None].clone()]
+    tokens, chosen = (t.rng.integers(0, 2, t.total) for _ in range(2))
+    results = []
+    for (k, v), rows in ((small, i32(t.table)), (large, table)):
+        path, accepted, following = (torch.zeros(shape, dtype=I32, device="cuda") for shape in ((2, 12), (2,), (2,)))
+        flag = torch.zeros(1, dtype=I32, device="cuda")
+        kernels.keep_drafts(k, v, i32(np.concatenate(t.parents)), i32(tokens), i32(chosen), i32(t.begin), i32(t.context), rows, 2, 12, path,
+                            accepted, following, flag)
+        first = 0 if k is small[0] else at
+        kernels.copy_pages(k, v, [(first + int(t.table[1, 2]), first + int(t.table[0, 1]), 11)])
+        assert int(flag.item()) == 0
+        results.append((path.tolist(), accepted.tolist(), following.tolist()))
+    assert results[0] == results[1]
+    for one, other in zip(small, large):
+        assert torch.equal(one[0], other[0, at:])
+
+
 # ------------------------------------------------------------------------------------------- kept drafts, pages
 def caches(layers, pages, heads, page, dim, value_dim, dtype, rng):
     make = lambda d: torch.tensor(rng.normal(size=(layers, pages, heads, page, d)), dtype=torch.float32).to(dtype).cuda()      # noqa: E731
@@ -347,6 +501,67 @@ def test_copy_pages(heads, page, dim, value_dim, count, dtype):
     kernels.copy_pages(k, v, [])
     kernels.copy_pages(k, v, [(2, 2, page)])                   # a page onto itself
     assert torch.equal(k, want[0]) and torch.equal(v, want[1])
+
+
+def test_keep_drafts_refused_spans_have_no_path():
+    from celeg_b200 import kernels
+    rng = np.random.default_rng(0)
+    k, v = caches(1, 20, 1, 16, 8, 8, torch.bfloat16, rng)
+    before = k.clone(), v.clone()
+    for begin, context in (((0, 5, 9), (2 ** 31 - 1, 3)), ((0, 5, 9), (-1, 3)), ((0, 5, 9), (2 ** 31 - 200, 3)), ((0, 11, 12), (0, 3))):
+        path, accepted, following = (torch.full(shape, 99, dtype=I32, device="cuda") for shape in ((2, 10), (2,), (2,)))
+        flag = torch.zeros(1, dtype=I32, device="cuda")
+        tokens = np.zeros(12, dtype=np.int32)
+        kernels.keep_drafts(k, v, i32([-1, 0, 0, 0, 0, -1, 0, 0, 0, 0, 0, -1]), i32(tokens), i32(tokens + 1), i32(begin), i32(context),
+                            i32(np.arange(20)[None].repeat(2, 0)), 2, 10, path, accepted, following, flag)
+        assert int(flag.item()) == 4
+        assert path[0].tolist() == [-1] * 10 and accepted.tolist() == [0, 1] and following.tolist() == [-1, 1]
+        assert path[1].tolist() == [0] + [-1] * 9
+    # parents that are no tree: only children behind their parent count
+    tokens = i32([5, 5, 5, 5])
+    kernels.keep_drafts(k, v, i32([3, 1, 0, 9]), tokens, tokens, i32([0, 4]), i32([0]), i32(np.arange(20)[None]), 1, 10, path, accepted,
+                        following, flag)
+    assert path[0].tolist() == [0, 2] + [-1] * 8
+    before[0][0, 0, :, 1], before[1][0, 0, :, 1] = before[0][0, 0, :, 2], before[1][0, 0, :, 2]
+    assert torch.equal(k, before[0]) and torch.equal(v, before[1])
+
+
+def test_pages_and_scores_in_a_graph_on_another_stream():
+    from celeg_b200 import kernels
+    rng = np.random.default_rng(3)
+    k, v = caches(2, 40, 2, 16, 64, 64, torch.bfloat16, rng)
+    start = k.clone(), v.clone()
+    parents, tokens = i32([-1, 0, 0, 2, 3, 3]), i32([9, 1, 2, 3, 4, 5])
+    chosen, begin, context, table = i32([2, 0, 3, 5, 0, 7]), i32([0, 6]), i32([30]), i32([[4, 9, 2]])
+    path, accepted, following = (torch.zeros(shape, dtype=I32, device="cuda") for shape in ((1, 6), (1,), (1,)))
+    flag = torch.zeros(1, dtype=I32, device="cuda")
+    logits = torch.randn((6, 30000), device="cuda")
+    outs = [torch.zeros(6, device="cuda"), torch.zeros(6, device="cuda"), torch.zeros((6, 3), device="cuda"),
+            torch.zeros((6, 3), dtype=I32, device="cuda")]
+
+    def call():
+        kernels.token_logprobs(logits, 6, tokens, *outs)
+        kernels.keep_drafts(k, v, parents, tokens, chosen, begin, context, table, 1, 6, path, accepted, following, flag)
+        kernels.copy_pages(k, v, [(4, 20, 16), (9, 21, 3)])
+
+    call()
+    torch.cuda.synchronize()
+    want = [x.clone() for x in (k, v, path, accepted, following, *outs)]
+    assert path.tolist() == [[0, 2, 3, 5, -1, -1]] and following.item() == 7
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        call()
+    for _ in range(2):
+        k.copy_(start[0]), v.copy_(start[1])
+        for x in (path, accepted, following, *outs):
+            x.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            graph.replay()
+        side.synchronize()
+        for x, y in zip((k, v, path, accepted, following, *outs), want):
+            assert torch.equal(x, y)
 
 
 # --------------------------------------------------------------------------------------------- log probabilities
@@ -439,3 +654,23 @@ def test_token_logprobs_rows_without_a_distribution():
     assert top_tokens[2].tolist() == [9, 0, 1, 2] and top_tokens[3].tolist() == [0, 1, 2, 3]
     got, *_ = score(x[4:], [300], 0)
     assert np.isnan(got).all()
+
+
+def test_token_logprobs_rows_behind_32_bit_offsets():
+    rows, vocab = 66000, 65541
+    logits = torch.empty((rows, vocab), dtype=torch.bfloat16, device="cuda")
+    logits[:-3] = 0.0
+    logits[-3:] = torch.randn((3, vocab), device="cuda")
+    from celeg_b200 import kernels
+    tokens = torch.arange(rows, dtype=I32, device="cuda") % vocab
+    logprobs, entropy = torch.empty(rows, device="cuda"), torch.empty(rows, device="cuda")
+    top_logprobs, top_tokens = torch.empty((rows, 2), device="cuda"), torch.empty((rows, 2), dtype=I32, device="cuda")
+    kernels.token_logprobs(logits, rows, tokens, logprobs, entropy, top_logprobs, top_tokens)
+    assert bool(((logprobs[:-3] + np.log(vocab)).abs() < 1e-5).all()) and bool(((entropy[:-3] - np.log(vocab)).abs() < 1e-4).all())
+    assert bool((top_tokens[:-3] == torch.tensor([0, 1], device="cuda")).all())
+    x = logits[-3:].double().cpu().numpy()
+    for r in range(3):
+        log_p, want = plain.log_probabilities(x[r])
+        assert abs(logprobs[rows - 3 + r].item() - log_p[int(tokens[rows - 3 + r])]) < 1e-5
+        assert abs(entropy[rows - 3 + r].item() - want) < 1e-4
+        assert top_tokens[rows - 3 + r].tolist() == plain.best(x[r], 2).tolist()
