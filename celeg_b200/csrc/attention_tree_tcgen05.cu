@@ -129,22 +129,26 @@ __device__ __forceinline__ unsigned long long tree_visible(const TreeParams& p, 
 __device__ __forceinline__ bool not_finite(unsigned bf16_bits) { return (bf16_bits & 0x7f80u) == 0x7f80u; }
 
 // 32 scores of a row to their weights relative to `base` (scores times `to_log2`), packed in pairs of bfloat16; returns the sum
-// of the weights and takes the largest score along.
+// of the weights. LARGEST: finds the largest of these scores and the 32 behind them on the way.
+template <bool LARGEST>
 __device__ __forceinline__ float tree_weights(const float* sc, unsigned long long scale2, unsigned long long neg_base2, unsigned (&packed)[16],
                                               float& largest) {
     unsigned long long sums[4] = {0ull, 0ull, 0ull, 0ull};      // (0.0f, 0.0f) each
-    float tops[2] = {largest, largest};
+    float tops[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int j2 = 0; j2 < 16; ++j2) {
         float x0, x1, a, b;
-        tops[j2 & 1] = max3_f32(tops[j2 & 1], sc[2 * j2], sc[2 * j2 + 1]);
+        if (LARGEST) {
+            tops[0] = max3_f32(tops[0], sc[2 * j2], sc[2 * j2 + 1]);
+            tops[1] = max3_f32(tops[1], sc[32 + 2 * j2], sc[32 + 2 * j2 + 1]);
+        }
         unpack_f32x2(fma_f32x2(pack_f32x2(sc[2 * j2], sc[2 * j2 + 1]), scale2, neg_base2), x0, x1);
         asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(x0));
         asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(b) : "f"(x1));
         sums[j2 & 3] = add_f32x2(sums[j2 & 3], pack_f32x2(a, b));
         packed[j2] = pack_bf16_pair(a, b);                      // (key 2 j2 in the lower half)
     }
-    largest = fmaxf(tops[0], tops[1]);
+    if (LARGEST) largest = fmaxf(tops[0], tops[1]);
     float s0, s1;
     unpack_f32x2(add_f32x2(add_f32x2(sums[0], sums[1]), add_f32x2(sums[2], sums[3])), s0, s1);
     return s0 + s1;
@@ -476,9 +480,11 @@ __global__ void __launch_bounds__(kTtThreads, 1) attention_tree_tcgen05_kernel(c
                 }
                 // The weights are taken relative to the maximum of the blocks before, while this block's is found: waiting for it first
                 // cost 350 cycles a step. Where it turns out larger by more than kSlack, which is rare behind a row's first blocks, O
-                // and the sum are rescaled and the weights taken once more.
+                // and the sum are rescaled and the weights taken once more. (The warp's rows are asked before the second half's
+                // exponentials, which hide the answer: 256 rows x 64 keys take an SM 895 ns, 971 with the question at the end. Asking
+                // for the next block's scores there as well, or four teams of which each waits more, took 1,026 and 1,077.)
                 bool settled = __any_sync(0xffffffffu, used_max == -INFINITY);
-                float largest = -INFINITY, sum;
+                float largest = -INFINITY, sum = 0.0f;
                 if (settled) {
 #pragma unroll
                     for (int j = 0; j < kTtN; j += 2) largest = max3_f32(largest, sc[j], sc[j + 1]);
@@ -514,15 +520,14 @@ __global__ void __launch_bounds__(kTtThreads, 1) attention_tree_tcgen05_kernel(c
                     }
                     const float base = used_max == -INFINITY ? 0.0f : used_max;
                     const unsigned long long neg_base2 = pack_f32x2(-base, -base);
-                    largest = -INFINITY;
-                    sum = tree_weights(sc, scale2, neg_base2, packed, largest);
-                    tmem_store_16(row_base + L::p_column(n), packed);
-                    sum += tree_weights(sc + 32, scale2, neg_base2, packed, largest);
-                    tmem_store_16(row_base + L::p_column(n) + 16u, packed);
-                    if (settled) break;
+                    sum = tree_weights<true>(sc, scale2, neg_base2, packed, largest);
+                    raise = !settled && __any_sync(0xffffffffu, largest * to_log2 > used_max + kSlack);
                     settled = true;
-                    raise = __any_sync(0xffffffffu, largest * to_log2 > used_max + kSlack);
-                    if (!raise) break;
+                    if (raise) continue;
+                    tmem_store_16(row_base + L::p_column(n), packed);
+                    sum += tree_weights<false>(sc + 32, scale2, neg_base2, packed, largest);
+                    tmem_store_16(row_base + L::p_column(n) + 16u, packed);
+                    break;
                 }
                 if (!ok) break;
                 run_sum += sum;
