@@ -9,7 +9,9 @@
 // arrive as fast as they run: two requests of 24 nodes x 1,500 positions in float32 took 51 us, 36 with 4.)
 // Keys and values come as they are stored, by asynchronous copies where rows are whole 16-byte pieces: of bfloat16 the next tile
 // under this one's products, of float32 one tile at a time, which leaves room for twice as many blocks an SM (eight requests of
-// 32 nodes x 4,096 positions: 256 us, 378 with two tiles).
+// 32 nodes x 4,096 positions in two pieces: 256 us, 378 with two tiles).
+// Instructions and what waits between a tile's two products bound it: 21 TFLOP/s, of the 72 that its units have, where there are
+// eight requests of 32 nodes x 4,096 positions (196 us); two of 24 behind 1,500 take 37 us, of which the join's launch is a part.
 #include "attention_tree.cuh"
 #include "attention_tree_tcgen05.h"
 #include "tcgen05.cuh"
@@ -368,16 +370,31 @@ static int launch_join(const TreeParams& p, cudaStream_t stream) {
     return check_launch("attention_tree (join)");
 }
 
-// Into how many pieces the keys are cut. `problems`: (row tile, kv head, span)s; `steps`: tiles of keys of the longest. A round
+// Into how many pieces the keys are cut on the tensor cores, one block an SM. `problems`: (row tile, kv head, span)s; `steps`: tiles of keys of the longest. A round
 // of blocks costs its tiles and some `ends` more for a block's beginning and end. Up to `cluster` pieces meet in a cluster,
 // which costs little, but a cluster wants neighbouring SMs; more pieces, as many as scratch holds, want a second launch.
-static int tree_splits(long long problems, const TreeTile& tile, long long steps, long long room) {
+static int tree_splits_tcgen05(long long problems, const TreeTile& tile, long long steps, long long room) {
     long long best = 1, least = 0;
     for (long long splits = 1; splits <= 64 && splits <= steps && (splits <= tile.cluster || splits <= room); ++splits) {
         const long long at_once = splits <= tile.cluster ? tile.problems_at_once[splits] : 0;
         const long long rounds = at_once > 0 ? (problems + at_once - 1) / at_once : (problems * splits + tile.blocks - 1) / tile.blocks;
         const long long joining = splits == 1 ? 0 : splits <= tile.cluster ? 4 : 8;
         const long long cost = 4 * (rounds * ((steps + splits - 1) / splits + tile.ends) + joining) + splits;
+        if (splits == 1 || cost < least) best = splits, least = cost;
+    }
+    return (int)best;
+}
+
+// ... and for the general kernel, whose blocks, several an SM, follow one another as they end: all blocks' tiles, with `ends` more a
+// block, spread over the places, and the last block's behind them; a join costs about as much as a tile. (Eight requests of 32 nodes
+// behind up to 4,096 positions, float32, heads of 64: 196 us in the 9 pieces that it takes, 206 in 12, 220 in 16, 247 in 24; heads of
+// 256: 329, 379, 415, 497; two requests of 24 behind 1,500: 39 us in 9, 37 in the 12 that it takes, 40 in 16, 47 in 24.)
+static int tree_splits_simt(long long problems, int head_dim, long long steps, long long room) {
+    const double places = head_dim <= 64 ? 592 : head_dim <= 128 ? 296 : 148, ends = 3;
+    long long best = 1;
+    double least = 0;
+    for (long long splits = 1; splits <= 64 && splits <= steps && (splits == 1 || splits <= room); ++splits) {
+        const double cost = (double)problems * (steps + splits * ends) / places + (double)((steps + splits - 1) / splits) + ends + (splits > 1 ? 1 : 0);
         if (splits == 1 || cost < least) best = splits, least = cost;
     }
     return (int)best;
@@ -473,12 +490,17 @@ CELEG_API int celeg_attention_tree(const void* record) {
     const bool tensor_cores = act_dtype == kBFloat16 && tree_tcgen05_takes(p);
     const size_t size = act_dtype == kFloat32 ? 4 : 2;
     const bool pieces = head_dim * size % 16 == 0 && page_stride * size % 16 == 0 && (((size_t)a.k_cache | (size_t)a.v_cache) & 15) == 0;
-    TreeTile tile = {kSimtRows, 592, 2, 1, {0}};
-    if (tensor_cores) tile = tree_tcgen05_tile(p);
     const long long reach = window > 0 && (long long)window + max_nodes < max_keys ? (long long)window + max_nodes : max_keys;
-    p.splits = tree_splits((long long)spans * kv_heads * ((max_nodes * group + tile.rows - 1) / tile.rows), tile, (reach + 63) / 64,
-                           scratch ? (scratch_elements - 1) / (units * (head_dim + 2)) : 0);
-    if (p.splits <= tile.cluster) p.part_o = nullptr;
+    const long long steps = (reach + 63) / 64, room = scratch ? (scratch_elements - 1) / (units * (head_dim + 2)) : 0;
+    const long long heads = (long long)spans * kv_heads, rows = (long long)max_nodes * group;
+    if (tensor_cores) {
+        const TreeTile tile = tree_tcgen05_tile(p);
+        p.splits = tree_splits_tcgen05(heads * ((rows + tile.rows - 1) / tile.rows), tile, steps, room);
+        if (p.splits <= tile.cluster) p.part_o = nullptr;
+    } else {
+        p.splits = tree_splits_simt(heads * ((rows + kSimtRows - 1) / kSimtRows), head_dim, steps, room);
+        if (p.splits == 1) p.part_o = nullptr;
+    }
     p.part_ml = p.part_o ? scratch + (units * p.splits * head_dim + 1) / 2 * 2 : nullptr;      // (read as pairs)
     int code;
     if (tensor_cores)
