@@ -27,7 +27,7 @@
 // its words of ancestors; a value that is not finite is taken out there and added to the rows that do see it at the end (a weight
 // of zero times it would reach the others).
 //
-// The weights are rounded to bfloat16 for their product with V (the denominator adds them up before): 2^-9 of each, at random.
+// The weights are rounded to bfloat16 for their product with V (the denominator adds them up before): 2^-8 of each at most, at random.
 // Warps without rows take no exponentials.
 #include "attention_tree.cuh"
 #include "attention_tree_tcgen05.h"
