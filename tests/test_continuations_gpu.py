@@ -2,6 +2,8 @@
 kept and forked, against the same model fed token by token."""
 from __future__ import annotations
 
+import importlib
+
 import numpy as np
 import pytest
 import torch
@@ -55,6 +57,47 @@ def test_a_fork_goes_on_as_the_request_itself_would(tmp_path, name, dtype, promp
     engine.loaded.step.raise_on_device_error()
     engine.loaded.manager.check_invariants()
     assert all(group.pool.used_pages == 0 for group in engine.loaded.manager.groups)
+
+
+@pytest.mark.parametrize("design", ["ramosun", "kedesun", "naselorn", "liverax", "kodupel", "fovezen"])
+def test_forks_of_every_design_carry_its_caches_and_states(tmp_path, design):
+    """Windows whose first pages are gone, values of another size than keys or of none, matrix states, convolutions' tails, layers
+    that repeat with caches of their own."""
+    from celeg_b200.engine.loading import load_model
+    from celeg_b200.engine.step import StepEntry
+    module = importlib.import_module(f"{design}_models")
+    for name, (raw, seed) in module.CONFIGS.items():
+        folder = str(tmp_path / name)
+        module.write_model(folder, raw, seed)
+        loaded = load_model(folder, dtype="float32", max_requests=4, cache_tokens=1024, max_batched_tokens=512, max_context=512)
+        rng = np.random.default_rng(seed)
+        vocab = loaded.model.vocab_size
+        prompt, ways = rng.integers(0, vocab, 70).tolist(), rng.integers(0, vocab, (2, 9)).tolist()
+
+        def feed(request, tokens):
+            logits = loaded.step.run([StepEntry(request, tokens, list(range(len(tokens))))], auto_begin=True).clone()
+            loaded.step.raise_on_device_error()
+            return logits
+
+        want = []
+        for way in ways:
+            feed("alone", prompt[:41])
+            feed("alone", prompt[41:])
+            want.append(torch.cat([feed("alone", way[:3])] + [feed("alone", [token]) for token in way[3:]]))
+            loaded.step.end("alone")
+        feed("a", prompt[:41])
+        feed("a", prompt[41:])
+        loaded.step.fork("a", "b")
+        got = [[feed("a", ways[0][:3])], [feed("b", ways[1][:3])]]
+        for a, b in zip(ways[0][3:], ways[1][3:]):
+            got[1].append(feed("b", [b]))
+            got[0].append(feed("a", [a]))
+        loaded.manager.check_invariants()
+        for rows, whole in zip(got, want):
+            assert (torch.cat(rows) - whole).abs().max().item() <= 1e-4 * max(1.0, whole.abs().max().item()), name
+        loaded.step.end("a")
+        loaded.step.end("b")
+        assert all(group.pool.used_pages == 0 for group in loaded.manager.groups)
 
 
 def test_a_fork_refuses_what_it_cannot_hold(tmp_path):
