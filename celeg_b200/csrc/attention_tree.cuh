@@ -46,18 +46,19 @@ struct TreeSpan {
     int begin, nodes, context;
 };
 
-__device__ __forceinline__ TreeSpan tree_span(const TreeParams& p, int span) {
+// `report`: sets the error flag (once a launch is enough: a join asks again what its pieces' blocks have asked).
+__device__ __forceinline__ TreeSpan tree_span(const TreeParams& p, int span, bool report = true) {
     TreeSpan s;
     s.begin = p.span_begin[span];
     s.nodes = p.span_begin[span + 1] - s.begin;
     s.context = p.span_context[span];
     if (s.begin < 0 || s.nodes < 0 || s.begin > p.tokens - s.nodes || s.nodes > p.max_nodes || s.context < 0) {
-        if (s.nodes != 0) atomicExch(p.error_flag, 4);
+        if (report && s.nodes != 0) atomicExch(p.error_flag, 4);
         s.nodes = 0;
     }
     const long long places = (long long)p.table_stride * p.page_tokens;
     if (s.nodes > 0 && (long long)s.context + s.nodes > (places < kTreeMaxPlaces ? places : kTreeMaxPlaces)) {
-        atomicExch(p.error_flag, 2);
+        if (report) atomicExch(p.error_flag, 2);
         s.nodes = 0;
     }
     return s;
