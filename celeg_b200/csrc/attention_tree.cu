@@ -415,7 +415,7 @@ using namespace celeg_b200;
 
 // The arguments of the entry point, one record. q: [tokens, q_row_stride] with head h at columns h * head_dim; caches: one
 // layer's [pages, kv_heads, page_tokens, head_dim], page_stride elements from page to page; span_begin [spans + 1],
-// span_context [spans], ancestors [tokens, words] (words of 32 bits), block_table [spans, table_stride]; sinks [q_heads] or
+// span_context [spans], ancestors [tokens, words] (words of 32 bits), block_table [spans, table_columns], rows table_stride apart; sinks [q_heads] or
 // null; out [tokens, q_heads * head_dim]. max_nodes: no span has more nodes (error 4 else); max_keys: about as many keys as the
 // longest span has, which only the number of pieces follows. scratch: float32, any number of elements; the keys are cut into
 // no more pieces than it holds where these do not meet in a cluster.
@@ -431,6 +431,7 @@ struct TreeArguments {
     long long q_row_stride, page_stride, scratch_elements;
     int pages, words, table_stride, tokens, spans, max_nodes, max_keys, q_heads, kv_heads, head_dim, page_tokens, window, act_dtype;
     float scale, softcap;
+    int table_columns;
 };
 static_assert(sizeof(TreeArguments) == 192, "the record that kernels.py packs");
 
@@ -457,6 +458,7 @@ CELEG_API int celeg_attention_tree(const void* record) {
     CELEG_REQUIRE(window >= 0 && softcap >= 0.0f && a.error_flag, "attention_tree: window %d, softcap %g, error_flag %p", window,
                   softcap, (void*)a.error_flag);
     CELEG_REQUIRE(act_dtype == kFloat32 || act_dtype == kBFloat16, "attention_tree: unknown dtype code %d", act_dtype);
+    CELEG_REQUIRE(a.table_stride >= 0 && a.table_columns >= 0, "attention_tree: a table of %d columns, rows %d apart", a.table_columns, a.table_stride);
     if (tokens == 0 || spans == 0) return 0;
     const int group = q_heads / kv_heads;
     const long long tiles = ((long long)max_nodes * group + 31) / 32;
@@ -477,6 +479,7 @@ CELEG_API int celeg_attention_tree(const void* record) {
     p.words = words;
     p.block_table = a.block_table;
     p.table_stride = a.table_stride;
+    p.table_columns = a.table_columns;
     p.tokens = tokens;
     p.spans = spans;
     p.max_nodes = max_nodes;

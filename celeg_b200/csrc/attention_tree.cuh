@@ -28,7 +28,7 @@ struct TreeParams {
     const int* span_begin;         // [spans + 1]
     const int* span_context;       // [spans]
     const unsigned* ancestors;     // [tokens, words]
-    const int* block_table;        // [spans, table_stride]
+    const int* block_table;        // [spans, table_columns], rows table_stride apart
     int words, table_stride, pages, tokens, spans, max_nodes;
     int q_heads, kv_heads, group, head_dim, page_tokens, window, splits;
     int page_shift;                // page_tokens = 1 << page_shift, -1: no power of two
@@ -38,6 +38,7 @@ struct TreeParams {
     float* part_o;                 // [tokens, q_heads, splits, head_dim]; null with one split
     float* part_ml;                // [tokens, q_heads, splits, 2]: maximum in units of log2, denominator
     int* error_flag;
+    int table_columns;             // (behind the others: in their midst, eight ragged requests took 27.5 us instead of 26.9)
 };
 
 // One span as a block sees it; nodes 0 where the block has nothing to do, or must not begin: a span outside the launch's sizes
@@ -56,7 +57,7 @@ __device__ __forceinline__ TreeSpan tree_span(const TreeParams& p, int span, boo
         if (report && s.nodes != 0) atomicExch(p.error_flag, 4);
         s.nodes = 0;
     }
-    const long long places = (long long)p.table_stride * p.page_tokens;
+    const long long places = (long long)p.table_columns * p.page_tokens;
     if (s.nodes > 0 && (long long)s.context + s.nodes > (places < kTreeMaxPlaces ? places : kTreeMaxPlaces)) {
         if (report) atomicExch(p.error_flag, 2);
         s.nodes = 0;
@@ -67,7 +68,7 @@ __device__ __forceinline__ TreeSpan tree_span(const TreeParams& p, int span, boo
 // The page that holds `place` of a span, -1 (and error 2) where there is none.
 __device__ __forceinline__ int tree_page(const TreeParams& p, const int* table, int place) {
     const int logical = place / p.page_tokens;
-    const int page = logical < p.table_stride ? table[logical] : -1;
+    const int page = logical < p.table_columns ? table[logical] : -1;
     if (page < 0 || page >= p.pages) {
         atomicExch(p.error_flag, 2);
         return -1;

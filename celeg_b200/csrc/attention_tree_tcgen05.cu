@@ -292,7 +292,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) attention_tree_tcgen05_kernel(c
             const int first_page = block_begin * kTtN >> p.page_shift, last_page = last_key >> p.page_shift, in_page = p.page_tokens - 1;
             auto entries = [&](int round) -> int {
                 const int logical = first_page + round * 32 + lane;
-                return logical <= last_page && logical < p.table_stride ? table[logical] : -1;
+                return logical <= last_page && logical < p.table_columns ? table[logical] : -1;
             };
             const unsigned stride = (unsigned)p.page_stride;    // (fits: see tree_tcgen05_takes)
             int held = entries(0), ahead = entries(1), round = 0;
@@ -332,7 +332,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) attention_tree_tcgen05_kernel(c
                 const int key = (block_begin + i) * kTtN + u * 32 + lane;
                 if (i >= blocks || key < first_key || key > last_key) return -2;
                 const int logical = key / p.page_tokens;
-                return logical < p.table_stride ? table[logical] : -1;
+                return logical < p.table_columns ? table[logical] : -1;
             };
             int page[2] = {look_up(pair, 0), look_up(pair, 1)};
             for (int i = pair; i < blocks; i += 2) {
@@ -606,7 +606,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) attention_tree_tcgen05_kernel(c
                         for (unsigned long long seen = tree_visible(p, s, mask, position, key_base); seen; seen &= seen - 1) {
                             const int key = key_base + __ffsll((long long)seen) - 1;
                             const int logical = key / p.page_tokens;
-                            const int page = logical < p.table_stride ? table[logical] : -1;
+                            const int page = logical < p.table_columns ? table[logical] : -1;
                             if (page < 0 || page >= p.pages) continue;
                             const __nv_bfloat16* v = static_cast<const __nv_bfloat16*>(p.v_cache) + (long long)page * p.page_stride +
                                                      ((long long)kvh * p.page_tokens + key % p.page_tokens) * d + c0;

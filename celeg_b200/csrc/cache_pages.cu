@@ -119,8 +119,8 @@ struct KeepParams {
     const int* chosen;             // [tokens]: what the model continues each node with
     const int* span_begin;
     const int* span_context;
-    const int* block_table;        // [spans, table_stride]
-    int table_stride, pages, token_count, layers, kv_heads, page_tokens, max_nodes;
+    const int* block_table;        // [spans, table_columns], rows table_stride apart
+    int table_stride, table_columns, pages, token_count, layers, kv_heads, page_tokens, max_nodes;
     int* path;                     // [spans, max_nodes], -1 behind the accepted nodes
     int* accepted;                 // [spans]
     int* next_token;               // [spans], -1 for a span without nodes
@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(kKeepThreads) keep_drafts_kernel(const KeepPar
         bool found = true;
         for (int e = 0; e < 2; ++e) {
             const int logical = place[e] / p.page_tokens;
-            const int page = logical < p.table_stride ? table[logical] : -1;
+            const int page = logical < p.table_columns ? table[logical] : -1;
             found = found && page >= 0 && page < p.pages;
             at[e][0] = page * p.k.page_stride + (long long)(place[e] % p.page_tokens) * p.k.row;
             at[e][1] = page * p.v.page_stride + (long long)(place[e] % p.page_tokens) * p.v.row;
@@ -310,7 +310,7 @@ CELEG_API int celeg_keep_drafts(const void* record) {
         int *path, *accepted, *next_token, *error_flag;
         cudaStream_t stream;
         long long strides[4];
-        int sizes[7], token_count, table_stride, spans, max_nodes;
+        int sizes[7], token_count, table_stride, spans, max_nodes, table_columns;
     } a;
     static_assert(sizeof(a) == 184, "the record that kernels.py packs");
     memcpy(&a, record, sizeof(a));
@@ -323,6 +323,8 @@ CELEG_API int celeg_keep_drafts(const void* record) {
                   kv_heads, page_tokens, k_dim, v_dim, element_bytes);
     CELEG_REQUIRE(spans >= 0 && spans <= 65535 && max_nodes >= 1 && max_nodes <= kKeepMaxNodes && a.error_flag,
                   "keep_drafts: %d spans of up to %d nodes (at most 65535 and %d)", spans, max_nodes, kKeepMaxNodes);
+    CELEG_REQUIRE(a.table_stride >= 0 && a.table_columns >= 0, "keep_drafts: a table of %d columns, rows %d apart", a.table_columns,
+                  a.table_stride);
     if (spans == 0) return 0;
     KeepParams p = {};
     p.k = cache_side(a.k, a.strides[0], a.strides[1], k_dim, element_bytes);
@@ -334,6 +336,7 @@ CELEG_API int celeg_keep_drafts(const void* record) {
     p.span_context = a.span_context;
     p.block_table = a.block_table;
     p.table_stride = a.table_stride;
+    p.table_columns = a.table_columns;
     p.pages = pages;
     p.token_count = token_count;
     p.layers = layers;

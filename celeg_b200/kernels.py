@@ -853,6 +853,8 @@ MAX_TOP_LOGPROBS = 128
 _TREE_RECORD = struct.Struct("=13Q3q13i2f4x")
 _COPY_RECORD = struct.Struct("=4Q4q8i")
 _KEEP_RECORD = struct.Struct("=13Q4q11i4x")
+# ... and the entries of a row of the block table at the end (a record that is packed without them refuses every span)
+_TREE_RECORD_WITH_TABLE, _KEEP_RECORD_WITH_TABLE = (struct.Struct(part.format[:-2] + "i") for part in (_TREE_RECORD, _KEEP_RECORD))
 _LOGPROBS_RECORD = struct.Struct("=7Qq4i")
 
 
@@ -890,8 +892,8 @@ def _check_vectors(operator: str, device: int, vectors) -> None:
 
 def _check_table(operator: str, table: torch.Tensor, spans: int) -> None:
     shape = table.shape
-    if len(shape) != 2 or shape[0] < spans or table.dtype is not _I32 or table.stride(1) != 1:
-        _refuse(f"{operator}: a block table {tuple(table.shape)} of {table.dtype} for {spans} spans")
+    if len(shape) != 2 or shape[0] < spans or table.dtype is not _I32 or (table.stride(1) != 1 and shape[1] > 1):
+        _refuse(f"{operator}: a block table {tuple(table.shape)} of {table.dtype} with strides {table.stride()} for {spans} spans")
 
 
 def attention_tree_scratch(device) -> torch.Tensor:
@@ -952,11 +954,11 @@ def attention_tree(q: torch.Tensor, q_row_stride: int, out: torch.Tensor, k_cach
     if scratch is not None and (scratch.dtype is not torch.float32 or not scratch.is_contiguous() or scratch.get_device() != device):
         _check_vectors(name, device, (("scratch", scratch, 0, torch.float32),))
     _check(library().celeg_attention_tree(_record(
-        name, _TREE_RECORD, q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), positions.data_ptr(),
+        name, _TREE_RECORD_WITH_TABLE, q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), positions.data_ptr(),
         span_begin.data_ptr(), span_context.data_ptr(), ancestors.data_ptr(), block_table.data_ptr(), _address(sinks),
         _address(scratch), error_flag.data_ptr(), _stream(), q_row_stride, strides[0], scratch.numel() if scratch is not None else 0,
         shape[0], masks[1], block_table.stride(0), tokens, spans, max_nodes, max_keys, q_heads, kv_heads, head_dim, page_tokens,
-        window or 0, code, scale, softcap or 0.0)))
+        window or 0, code, scale, softcap or 0.0, block_table.shape[1])))
 
 
 def _cache_sides(operator: str, k: torch.Tensor, v: torch.Tensor) -> tuple:
@@ -1030,9 +1032,9 @@ def keep_drafts(k: torch.Tensor, v: torch.Tensor, parents: torch.Tensor, tokens:
             ("path", path, spans * max_nodes, _I32), ("accepted", accepted, spans, _I32), ("next_token", next_token, spans, _I32),
             ("error_flag", error_flag, 1, _I32)))
     _check(library().celeg_keep_drafts(_record(
-        name, _KEEP_RECORD, keys, values, parents.data_ptr(), tokens.data_ptr(), chosen.data_ptr(), span_begin.data_ptr(),
+        name, _KEEP_RECORD_WITH_TABLE, keys, values, parents.data_ptr(), tokens.data_ptr(), chosen.data_ptr(), span_begin.data_ptr(),
         span_context.data_ptr(), block_table.data_ptr(), path.data_ptr(), accepted.data_ptr(), next_token.data_ptr(),
-        error_flag.data_ptr(), _stream(), *sizes, count, block_table.stride(0), spans, max_nodes)))
+        error_flag.data_ptr(), _stream(), *sizes, count, block_table.stride(0), spans, max_nodes, block_table.shape[1])))
 
 
 def token_logprobs(logits: torch.Tensor, rows: int, tokens: Optional[torch.Tensor], logprobs: Optional[torch.Tensor],
