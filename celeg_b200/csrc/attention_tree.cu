@@ -283,12 +283,12 @@ __global__ void __launch_bounds__(kSimtThreads) attention_tree_simt_kernel(const
                 p.part_ml[(unit * p.splits + split) * 2] = run_max[i] * 1.4426950408889634f;
                 p.part_ml[(unit * p.splits + split) * 2 + 1] = sum;
             }
-            if (run_max[i] == -INFINITY) continue;
+            if (run_max[i] == -INFINITY && sum == 0.0f) continue;       // (no key; a sum of NaN: scores of NaN, which maxima leave out)
         }
         float inv = 1.0f;
         if (p.splits == 1) {
             if (p.sinks && sum > 0.0f) sum += expf(p.sinks[head] - run_max[i]);
-            inv = run_max[i] == -INFINITY ? 0.0f : 1.0f / sum;
+            inv = run_max[i] == -INFINITY ? sum : 1.0f / sum;           // (0, or NaN)
         }
 #pragma unroll
         for (int j = 0; j < COLUMNS; ++j) {
@@ -330,10 +330,11 @@ __global__ void __launch_bounds__(256) attention_tree_join_kernel(const TreePara
     }
     if (!there) return;
     const float top = warp_max(fmaxf(low.x, high.x));
-    const float low_factor = low.x == -INFINITY ? 0.0f : exp2f(low.x - top), high_factor = high.x == -INFINITY ? 0.0f : exp2f(high.x - top);
+    // (a piece without a maximum has a sum of 0, or of NaN where it saw NaN alone)
+    const float low_factor = low.x == -INFINITY ? low.y : exp2f(low.x - top), high_factor = high.x == -INFINITY ? high.y : exp2f(high.x - top);
     float total = warp_sum(low.y * low_factor + high.y * high_factor);
     if (p.sinks && top != -INFINITY) total += exp2f(p.sinks[unit % p.q_heads] * 1.4426950408889634f - top);
-    const float inv = top == -INFINITY ? 0.0f : 1.0f / total;
+    const float inv = top == -INFINITY ? total : 1.0f / total;
     for (int c = lane; c < d + lane; c += 32) {        // (every lane comes to every exchange)
         float sum = 0.0f;
         for (int i0 = 0; i0 < p.splits; i0 += 4) {

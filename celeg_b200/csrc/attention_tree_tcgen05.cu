@@ -644,7 +644,8 @@ __global__ void __launch_bounds__(kTtThreads, 1) attention_tree_tcgen05_kernel(c
 #pragma unroll 1
         for (int part = 0; part < parts; ++part) {
             const float2 stats = row_stats[part * most + tid];
-            const float factor = stats.x == -INFINITY ? 0.0f : fast_exp2(stats.x - top);
+            // (a part without a maximum has a sum of 0, or of NaN where it saw NaN alone: maxima leave that out, rows must not)
+            const float factor = stats.x == -INFINITY ? stats.y : fast_exp2(stats.x - top);
             sum = fmaf(stats.y, factor, sum);
             row_stats[part * most + tid].x = factor;
         }
@@ -656,7 +657,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) attention_tree_tcgen05_kernel(c
             *reinterpret_cast<float2*>(p.part_ml + ((size_t)unit * p.splits + split) * 2) = make_float2(top, sum);
         } else {
             if (p.sinks && top != -INFINITY) sum += fast_exp2(p.sinks[of_head] * 1.4426950408889634f - top);
-            inv = top == -INFINITY ? 0.0f : 1.0f / sum;
+            inv = top == -INFINITY ? sum : 1.0f / sum;
         }
 #pragma unroll 1
         for (int part = 0; part < parts; ++part) row_stats[part * most + tid].y = inv;

@@ -913,8 +913,9 @@ def attention_tree(q: torch.Tensor, q_row_stride: int, out: torch.Tensor, k_cach
     positions and, behind them, node j at place span_context[s] + j (keys and values already stored). A node sees the cached
     positions and the nodes whose bits its row of ``ancestors`` has (int32 [tokens, words], bit j % 32 of word j // 32; a node
     sees itself only with its own bit), of these under a ``window`` those less than that many positions before its own:
-    ``positions`` [tokens] are the nodes' positions, a cached place's is itself. A row that sees nothing is zeros. Rows behind the last
-    span, and of a span that reaches past its row of the table (error 2) or the launch's sizes (error 4), stay as they were.
+    ``positions`` [tokens] are the nodes' positions, a cached place's is itself. A row that sees nothing, or only keys whose scores
+    are -inf, is zeros, one that sees a score of NaN is NaN. Rows behind the last span, and of a span that reaches past its row of the
+    table (error 2) or the launch's sizes (error 4), stay as they were.
     ``q`` [tokens, *] with head h at column h * head_dim, rows ``q_row_stride`` apart; ``out`` [tokens, q_heads * head_dim];
     caches: one layer's pages. ``sinks``, ``softcap``: as for :func:`attention_generic`. ``max_keys``: about the longest span's
     cached positions and nodes; with ``scratch`` (:func:`attention_tree_scratch`, or any float32 vector) long contexts are cut
