@@ -106,7 +106,8 @@ __global__ void attention_generic_kernel(const A* __restrict__ q, int q_row_stri
         }
         const float block_max = warp_max(score);
         const float new_max = fmaxf(running_max, block_max);
-        if (new_max == -INFINITY) continue;          // nothing readable in this block of keys
+        // nothing readable in this block of keys; scores of NaN alone, which a maximum leaves out, go on and make the row NaN
+        if (new_max == -INFINITY && !__any_sync(0xffffffffu, score != score)) continue;
         const float correction = expf(running_max - new_max);   // exp(-inf) = 0 on the first block
         const float p = score == -INFINITY ? 0.0f : expf(score - new_max);
         denom = denom * correction + warp_sum(p);
