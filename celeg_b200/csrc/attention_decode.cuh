@@ -487,8 +487,9 @@ __device__ __forceinline__ void attention_decode_item(const DecodeParams& p, con
         const float sink_log2 = with_sink ? p.sinks[kvh * group + tid] * 1.4426950408889634f : -INFINITY;
         m = fmaxf(m, sink_log2);
         float sum = with_sink ? exp2f(sink_log2 - m) : 0.0f;
+        // (a warp without a maximum has a sum of 0, or of NaN where it saw NaN alone, which maxima leave out)
         for (int w = 0; w < kDecodeWarps; ++w)
-            sum += warp_max_s[w][tid] == -INFINITY ? 0.0f : warp_sum_s[w][tid] * exp2f(warp_max_s[w][tid] - m);
+            sum += warp_max_s[w][tid] == -INFINITY ? warp_sum_s[w][tid] : warp_sum_s[w][tid] * exp2f(warp_max_s[w][tid] - m);
         head_max[tid] = m;
         head_sum[tid] = sum;
     }
