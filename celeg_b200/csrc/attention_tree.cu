@@ -11,7 +11,8 @@
 // under this one's products, of float32 one tile at a time, which leaves room for twice as many blocks an SM (eight requests of
 // 32 nodes x 4,096 positions in two pieces: 256 us, 378 with two tiles).
 // Instructions and what waits between a tile's two products bound it: 21 TFLOP/s, of the 72 that its units have, where there are
-// eight requests of 32 nodes x 4,096 positions (196 us); two of 24 behind 1,500 take 37 us, of which the join's launch is a part.
+// eight requests of up to 32 nodes x 4,096 positions on 32 heads of 64 (194 us); two of up to 24 behind 1,500 take 37 us, of which
+// the join's launch is a part.
 #include "attention_tree.cuh"
 #include "attention_tree_tcgen05.h"
 #include "tcgen05.cuh"
@@ -397,8 +398,8 @@ static int tree_splits_tcgen05(long long problems, const TreeTile& tile, long lo
 
 // ... and for the general kernel, whose blocks, several an SM, follow one another as they end: all blocks' tiles, with `ends` more a
 // block, spread over the places, and the last block's behind them; a join costs about as much as a tile. (Eight requests of 32 nodes
-// behind up to 4,096 positions, float32, heads of 64: 196 us in the 9 pieces that it takes, 206 in 12, 220 in 16, 247 in 24; heads of
-// 256: 329, 379, 415, 497; two requests of 24 behind 1,500: 39 us in 9, 37 in the 12 that it takes, 40 in 16, 47 in 24.)
+// behind up to 4,096 positions, float32, heads of 64: 196 us in the 9 pieces that it takes, 206 in 12, 220 in 16, 247 in 24; 8 heads
+// of 256: 329, 379, 415, 497; two requests of 24 behind 1,500: 39 us in 9, 37 in the 12 that it takes, 40 in 16, 47 in 24.)
 static int tree_splits_simt(long long problems, int head_dim, long long steps, long long room) {
     const double places = head_dim <= 64 ? 592 : head_dim <= 128 ? 296 : 148, ends = 3;
     long long best = 1;

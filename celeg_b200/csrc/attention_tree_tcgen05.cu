@@ -19,9 +19,10 @@
 //
 // What bounds it: where blocks of keys are many, the softmax. An SM takes 16 exponentials a cycle, 512 cycles for 128 rows x 64
 // keys, and the step of a team (scores from tensor memory, scaling, exponentials, packing, weights to tensor memory) is a chain
-// that two teams cover to 850 cycles. Four trees of 64 nodes on 32 heads of 64 behind 65,536 positions: 236 us, 580 TFLOP/s,
-// 2.3 TB/s. Where they are few, the chain from the launch to the last store, about 9 us: one tree of 13 nodes behind 601 positions
-// 9.4 us. Eight trees of up to 32 nodes behind 1,161 to 4,096 positions, in clusters of two: 26 us, as long as the longest takes.
+// that two teams cover to 850 cycles. Four trees of 64 nodes on 32 heads of 64 behind 65,536 positions: 239 us, 575 TFLOP/s,
+// 2.3 TB/s, the special-function pipe at 59 % and the tensor pipe at 29 % of their rates. Where they are few, the chain from the launch to the last store, about 9 us: one tree of 13 nodes behind 601 positions
+// 9.7 us. Eight trees of up to 32 nodes behind 1,161 to 4,096 positions, in clusters of two: 27 us, as long as the longest takes.
+// (Times in a graph, inputs in turn.)
 //
 // Blocks of keys before the tree are seen whole by every row and need no mask. In the others a row's mask is 64 bits, cut from
 // its words of ancestors; a value that is not finite is taken out there and added to the rows that do see it at the end (a weight

@@ -28,8 +28,8 @@ constexpr int kFewMoves = 32, kManyMoves = 1024;
 
 // One (move, layer) a block in x, keys or values in y. V: what a thread moves at a time; four of them are under way. A page of 16
 // positions x 8 heads x 64 is 16 KiB, a pass of 256 threads: every block asks for all that it moves at once. 768 pages in sixteen
-// layers, keys and values (805 MB read and written together), take 124 us, 6,490 GB/s, what a copy reaches here; a fork's one
-// page in six layers 1.6 us, a launch.
+// layers, keys and values (805 MB read and written together), take 125 us, 6,440 GB/s, what a copy reaches here; a fork's one
+// page in six layers 1.9 us, a launch.
 template <typename V, int N>
 __global__ void __launch_bounds__(256) copy_pages_kernel(const __grid_constant__ PageMoves<N> moves, const int layers, const CacheSide k,
                                                          const CacheSide v, const int kv_heads, const int page_tokens) {
@@ -131,8 +131,8 @@ struct KeepParams {
 // and moves it for the whole path, in order. Path nodes rise and node n of the path is n or later, so that a row is read
 // before its place is written, within the thread that does both; no row is another thread's.
 // Every block walks the tree for itself, one warp with up to eight nodes a lane: a step is a ballot of "child of the current node with the
-// chosen token" over each 32 nodes, the lowest wins. The chain of reads, span, tree, table, rows, is what bounds it: 3.4 us for one
-// request in six layers, 4.9 us for 64 of 32 drafts in sixteen (8.4 MB, 1.3 us at the memory's rate).
+// chosen token" over each 32 nodes, the lowest wins. The chain of reads, span, tree, table, rows, is what bounds it: 3.8 us for one
+// request in six layers, 5.1 us for 64 of 32 drafts in sixteen (8.4 MB, 1.3 us at the memory's rate).
 template <typename V>
 __global__ void __launch_bounds__(kKeepThreads) keep_drafts_kernel(const KeepParams p) {
     __shared__ int path_s[kKeepMaxNodes];

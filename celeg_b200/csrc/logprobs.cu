@@ -16,8 +16,8 @@
 // first block, where everything a block has meets.
 //
 // Over many rows the logits' bytes are what bounds it: 4,095 rows of 65,536 float32 logits take 162 us, 6,630 GB/s (in bfloat16
-// 149 us: there the instructions a logit do). Of few rows, the chain of a block's reductions: 8.2 us for one row of 65,536 with its
-// twenty best, 10.3 us for 64 of 50,257 with five.
+// 151 us: there the instructions a logit do). Of few rows, the chain of a block's reductions: 8.5 us for one row of 65,536 with its
+// twenty best, 11 us for 64 of 50,257 with five.
 #include "common.cuh"
 #include "tcgen05.cuh"
 

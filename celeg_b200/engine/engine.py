@@ -257,7 +257,8 @@ class Engine:
         """How likely the model finds given tokens: for every prompt a :class:`TokenScores` with the log probability of each
         token behind the first, given those before it, the entropy of the distribution it was taken from and, with
         ``top`` (at most 128), the most likely tokens there. One prompt gives one, several give a list. Needs a free
-        state slot and pages for one prompt at a time; unscaled logits (temperature 1, no penalties)."""
+        state slot and pages for one prompt at a time; unscaled logits (temperature 1, no penalties). A prompt is scored in one
+        go: requests that a worker thread decodes wait until it is done."""
         if isinstance(prompts, (np.ndarray, torch.Tensor)):
             prompts = prompts.tolist()
         single = len(prompts) > 0 and not isinstance(prompts[0], (list, tuple, np.ndarray, torch.Tensor))

@@ -897,8 +897,9 @@ def _check_table(operator: str, table: torch.Tensor, spans: int) -> None:
 
 
 def attention_tree_scratch(device) -> torch.Tensor:
-    """Scratch of :func:`attention_tree` with room for as many pieces as it cuts the keys into at any size; one for all layers
-    of a model, or for all calls that follow one another on a stream."""
+    """Scratch of :func:`attention_tree`, 64 MB: room for 2^24 / (tokens * q_heads * (head_dim + 2)) pieces of the keys. A step that
+    would take more is cut into as many as fit; a larger float32 vector serves as well. One for all layers of a model, or for all
+    calls that follow one another on a stream."""
     return torch.empty(1 << 24, dtype=torch.float32, device=device)
 
 
@@ -1043,8 +1044,8 @@ def token_logprobs(logits: torch.Tensor, rows: int, tokens: Optional[torch.Tenso
                    top_tokens: Optional[torch.Tensor] = None) -> None:
     """logprobs[r] = log softmax(logits[r])[tokens[r]] in nats, ``entropy`` [rows] of the same distributions, and the
     ``top_tokens`` [rows, k <= 128] (int32) with the largest logits, largest first, equal ones by the lower index, with their
-    log probabilities (csrc/logprobs.cu). ``logits``: float32 or bfloat16 [rows, vocab], rows at any stride; the results are
-    float32. A token outside the vocabulary has the log probability NaN; so have all of a row with a NaN, without a logit
+    log probabilities (csrc/logprobs.cu). ``logits``: float32 or bfloat16 [rows, vocab], rows ``vocab`` or more numbers apart;
+    the results are float32. A token outside the vocabulary has the log probability NaN; so have all of a row with a NaN, without a logit
     above -inf or with one of +inf (a NaN counts as the smallest logit). Outputs that are None are left out."""
     name = "token_logprobs"
     code = dtype_code(logits.dtype)
